@@ -115,6 +115,23 @@ class GatedDelta(C.Structure):
                [(n, _P) for n in ("a2", "g2", "rate", "dt_bias", "u")] + [("ld_u", _U), ("decay", _P), ("gate", _P), ("ld_decay", _U), ("ld_gate", _U)]
 
 
+class PagedCache(C.Structure):
+    _fields_ = [("fmt", C.c_int), ("k", _P), ("v", _P)] + [(n, _U) for n in ("pages", "kv_heads", "page", "dim")] + [("table", _P), ("ld_table", _U)]
+
+
+class Ragged(C.Structure):
+    _fields_ = [(n, _U) for n in ("batch", "tokens", "max_rows")] + [("start", _P), ("len", _P)]
+
+
+class Rotation(C.Structure):
+    _fields_ = [("dims", _U), ("interleaved", C.c_int), ("base", C.c_double), ("freq", _P), ("amplitude", _F)]
+
+
+class LogitsRules(C.Structure):
+    _fields_ = [("ids", _P), ("ld_ids", _U)] + [(n, _P) for n in ("n_ids", "n_prompt", "repetition", "frequency", "presence", "bias_ids", "bias", "bias_start", "allowed")] + \
+               [("ld_allowed", _U)]
+
+
 def cuda():
     return _load("libgreta_cuda.so", "greta_cuda.h")
 

@@ -428,6 +428,89 @@ GRETA_API int greta_cuda_kv_update(greta_stream_t stream, void *k_cache_f16, voi
 GRETA_API int greta_cuda_rope_kv(greta_stream_t stream, float *q, const float *k, const float *v, void *kc, void *vc, uint32_t S, uint32_t H, uint32_t Hkv,
                                  uint32_t Dh, float base, uint32_t pos, uint32_t max_seq);
 
+/* ------------------------------------------------------------------ paged caches, ragged batches
+ * The operators of a serving step whose sequences share one pool of cache pages and bring any number of new tokens each: portions of
+ * prompts, drafted tokens, single decode tokens, mixed in one call.  New with this build: the reference holds one sequence in one
+ * contiguous cache (src/inference/src/block_scheduler.cpp:1490-1494).
+ *
+ * Position p of sequence b lies in page table[b * ld_table + p / page], at row p % page.  A page of the k pool (and of the v pool) is
+ * [kv_heads][page][dim].  A table entry outside 0 .. pages - 1 is no page: nothing is written there, and its keys and values count as
+ * rows of zeros.  dim: a multiple of 8 up to 128; page: a power of two from 8 to 256; pages * kv_heads * page below 2^31; k and v
+ * 16-byte aligned. */
+typedef struct greta_paged_cache {
+  int fmt; /* GRETA_FMT_F16 or GRETA_FMT_BF16 */
+  void *k, *v;
+  uint32_t pages, kv_heads, page, dim;
+  const int32_t *table; /* device, [batch][ld_table] */
+  uint32_t ld_table;
+} greta_paged_cache;
+/* Sequence b has rows start[b] .. start[b + 1] - 1 of the token buffers and len[b] positions, these rows being the last of them: row i of
+ * r is at position len[b] - r + i (a row whose position would be negative has none: paged_append passes it over, paged_attn
+ * gives it zeros).  Both arrays are read on the device when the call runs; start does not decrease, starts and lengths are taken as at most
+ * tokens and ld_table * page.  Rows that belong to no sequence are left as they are.  batch: 1 to 1024. */
+typedef struct greta_ragged {
+  uint32_t batch, tokens; /* tokens: rows of the buffers, an upper bound of start[batch] */
+  uint32_t max_rows;      /* upper bound of a sequence's rows, rows behind it are not looked at; 0 = tokens */
+  const uint32_t *start;  /* device, [batch + 1] */
+  const uint32_t *len;    /* device, [batch] */
+} greta_ragged;
+/* Pairs of the first `dims` elements of a head are turned by position * freq[i], i < dims / 2: elements i and i + dims / 2, or with
+ * `interleaved` 2 i and 2 i + 1; cosine and sine are multiplied by `amplitude`.  The angle is taken modulo a turn in 64-bit integers, so far positions turn
+ * as exactly as near ones.  dims: even, at most dim, 0 = no rotation.  freq: host memory, read during the call; NULL = base^(-2 i / dims). */
+typedef struct greta_rotation {
+  uint32_t dims;
+  int interleaved;
+  double base;
+  const double *freq;
+  float amplitude;
+} greta_rotation;
+/* New rows of q [tokens][heads][dim], k and v [tokens][kv_heads][dim], all of type fmt (GRETA_FMT_F32, F16 or BF16): k rotated to the
+ * cache, v to the cache, q rotated to q_out (type q_fmt, any of the three; q_out may be q where types and ld agree).  q and q_out may
+ * be NULL together.  ld_*: elements from a token to the next.  Pointers 16-byte aligned, ld_* whole 16 bytes.  The ragged form of greta_cuda_rope_kv
+ * (launch_rope and launch_kv_update, attention_kernels.hip:28-158).  Two rows of one call at the same place of the cache: either is kept. */
+GRETA_API int greta_cuda_paged_append(greta_stream_t stream, const greta_paged_cache *cache, const greta_ragged *rows, const greta_rotation *rotation, int fmt,
+                                      const void *q, uint32_t ld_q, const void *k, uint32_t ld_k, const void *v, uint32_t ld_v, uint32_t heads, void *q_out,
+                                      int q_fmt, uint32_t ld_q_out);
+/* o = softmax(scale q k^T) v of every new row over the positions up to its own, with window > 0 over the last `window` of them.  q and o
+ * [tokens][heads][dim], both of type q_fmt: GRETA_FMT_F32 (products and sums keep fp32 precision), or the cache's type (probabilities are
+ * rounded to it, the rest is fp32).  heads: a multiple of kv_heads.  The new rows' keys and values are in the cache already (greta_cuda_paged_append).  What
+ * lies behind a row's position, or in front of its window, does not reach it whatever it is.  Rows without keys are zeros.  o and q do not overlap.
+ * workspace: greta_cuda_paged_attn_workspace_bytes(dim) bytes, 16-byte aligned, its first 64 KB zero before the first call; one serves every
+ * shape, one call at a time.  Waits in the kernels are bounded; one that gave up shows in greta_cuda_gemm_segments_status.
+ * The ragged form of greta_cuda_attn_decode_batch and greta_cuda_attn_prefill. */
+GRETA_API size_t greta_cuda_paged_attn_workspace_bytes(uint32_t dim);
+GRETA_API int greta_cuda_paged_attn(greta_stream_t stream, const greta_paged_cache *cache, const greta_ragged *rows, const void *q, int q_fmt, uint32_t ld_q,
+                                    void *o, uint32_t ld_o, uint32_t heads, float scale, uint32_t window, void *workspace, size_t workspace_bytes);
+
+/* ------------------------------------------------------------------ rules on logits
+ * What the text so far and the caller want of the next token.  Row m of the logits, value x of token t, in this order, fp32:
+ *   t among ids[m][0 .. n_ids[m] - 1]:  x > 0 ? x / repetition[m] : x * repetition[m]
+ *   c times among ids[m][n_prompt[m] ..]:  x - frequency[m] * c, and - presence[m] where c > 0
+ *   t among bias_ids[bias_start[m] .. bias_start[m + 1] - 1]:  + its bias (of a token listed more than once, the last)
+ *   bit t % 32 of allowed[m][t / 32] clear:  -infinity
+ * All arrays on the device; a NULL array is a rule left out (ids, bias_ids and allowed switch their groups off; n_prompt NULL: 0).  Ids outside the vocabulary are passed over. */
+typedef struct greta_logits_rules {
+  int32_t *ids; /* [M][ld_ids] */
+  uint32_t ld_ids;
+  uint32_t *n_ids;          /* [M], taken as at most ld_ids */
+  const uint32_t *n_prompt; /* [M] */
+  const float *repetition, *frequency, *presence; /* [M] each */
+  const int32_t *bias_ids;
+  const float *bias;
+  const uint32_t *bias_start; /* [M + 1] */
+  const uint32_t *allowed;    /* [M][ld_allowed] */
+  uint32_t ld_allowed;        /* words, at least V / 32 rounded up */
+} greta_logits_rules;
+/* out = the logits under the rules (type fmt: GRETA_FMT_F32, F16 or BF16, rounded once; may be the logits themselves, with the same ld; NULL:
+ * not wanted), d_next[m] = the first maximum of row m as it is written (greta_cuda_argmax's rules; NULL: not wanted).  ld, ld_out: elements between rows.  Stands in front of,
+ * or in the place of, launch_argmax (basic_kernels.hip:330-373). */
+GRETA_API int greta_cuda_logits_adjust(greta_stream_t stream, const greta_logits_rules *rules, int fmt, const void *logits, uint32_t ld, void *out,
+                                       uint32_t ld_out, uint32_t M, uint32_t V, int32_t *d_next);
+/* The same as the end of a decode step on the device: the chosen id is also appended to ids[m] (while there is room: n_ids[m] < ld_ids), n_ids[m] and, where
+ * d_pos is not NULL, d_pos[m] go up by one.  Needs d_next, ids and n_ids. */
+GRETA_API int greta_cuda_logits_adjust_advance(greta_stream_t stream, const greta_logits_rules *rules, int fmt, const void *logits, uint32_t ld, void *out,
+                                               uint32_t ld_out, uint32_t M, uint32_t V, int32_t *d_next, uint32_t *d_pos);
+
 /* ------------------------------------------------------------------ small operators */
 /* launch_rmsnorm_naive (basic_kernels.hip:21-64); also what GretaCompute::rmsnorm
  * (greta_compute_hip.cpp:414-419, an empty placeholder in the reference) calls. */
