@@ -203,14 +203,13 @@ extern "C" int greta_cuda_paged_append(greta_stream_t stream, const greta_paged_
   a.q_fmt = q_fmt;
   a.interleaved = rotation->interleaved != 0;
   a.amplitude = rotation->amplitude;
+  GRETA_REQUIRE(a.dims == 0 || rotation->freq || (rotation->base > 0 && std::isfinite(rotation->base)), "paged_append: base %g", rotation->base);
+  // Powers of base^(-2 / dims) by products: 63 roundings to 64 bits, and one powl instead of 64 (18 us of a call).
+  const long double step = a.dims && !rotation->freq ? powl((long double)rotation->base, -2.0L / a.dims) : 1.0L;
+  long double power = 1.0L;
   for (uint32_t i = 0; i < a.dims / 2; ++i) {
-    long double f;
-    if (rotation->freq) {
-      f = rotation->freq[i];
-    } else {
-      GRETA_REQUIRE(rotation->base > 0, "paged_append: base %g", rotation->base);
-      f = powl((long double)rotation->base, -2.0L * i / a.dims);
-    }
+    const long double f = rotation->freq ? (long double)rotation->freq[i] : power;
+    power *= step;
     GRETA_REQUIRE(std::isfinite((double)f), "paged_append: frequency %u is no finite number", i);
     const long double turns = f / 6.283185307179586476925286766559005768L, part = turns - floorl(turns);  // of a turn per position, 0 .. 1
     const long double scaled = part * 18446744073709551616.0L + 0.5L;

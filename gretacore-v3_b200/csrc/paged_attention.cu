@@ -25,6 +25,7 @@ using namespace greta;
 namespace {
 
 constexpr uint32_t PM_KEYS = 64, PM_WARPS = 4, PM_THREADS = 32 * (PM_WARPS + 1);
+constexpr uint32_t PM_LIST = 2;  // what a row block costs besides its tiles, in tiles: its queries, sums and outputs
 constexpr float PM_LOWEST = -3.4028234e38f;  // a row's maximum before any score: scores of minus infinity have weight 0 whatever stands in front of them
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -63,6 +64,10 @@ __device__ __forceinline__ void split(float a, float b, uint32_t (&w)[TERMS]) {
     }
   }
 }
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar) {  // 16-byte boundaries and sizes
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 __device__ __forceinline__ void bar_math() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 
 // What a CTA works on at a time: key tiles t0 .. t1 - 1 (absolute, of 64 keys) of 16 MT rows from R0 on of KV head g of sequence b.
@@ -82,9 +87,10 @@ struct PmShape {
   static constexpr uint32_t TILE = PM_KEYS * DH * 2;                 // bytes of a tile of keys, or values
   static constexpr uint32_t QP = DH * 2 + 16, PP = PM_KEYS * 2 + 16;  // bytes from a row to the next (16 more: ldmatrix rows in different banks)
   static constexpr uint32_t Q = MT > 1 ? TERMS * ROWS * QP : 0, P = TERMS * ROWS * PP;
+  static constexpr uint32_t RAW = DH * (F32 ? 4 : 2) + 16, QR = MT > 1 ? 0 : ROWS * RAW;  // queries as they come (one row block): by bulk copies, a block ahead
   static constexpr uint32_t RING = STAGES * 2 * TILE;
   static constexpr uint32_t MAXIMA = PM_WARPS * ROWS * 4;
-  static constexpr size_t bytes(uint32_t batch) { return 1024 + RING + Q + P + 2 * MAXIMA + ROWS * 4 + (size_t)(batch + 1) * 8 + 2 * STAGES * 8 + 32; }
+  static constexpr size_t bytes(uint32_t batch) { return 1024 + RING + Q + QR + P + 2 * MAXIMA + ROWS * 4 + (size_t)batch * 24 + 8 + (2 * STAGES + 1) * 8 + 16; }
 };
 
 // Tiles of a sequence's lists (all row blocks alike: those in front of a block's window or behind its last row are passed over), its blocks.
@@ -104,13 +110,14 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
   constexpr uint32_t DH = Z::DH, ROWS = Z::ROWS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *ring = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);  // [stage][keys, values][slab][64 rows of 128 bytes, swizzled]
-  uint8_t *qs = ring + Z::RING, *ps = qs + Z::Q;
+  uint8_t *qs = ring + Z::RING, *qr = qs + Z::Q, *ps = qr + Z::QR;
   float *maxima = reinterpret_cast<float *>(ps + Z::P);        // [warp][row]
   float *sums = maxima + PM_WARPS * ROWS;                      // [warp][row]
   float *factor = sums + PM_WARPS * ROWS;                      // [row]: what scores are multiplied by
-  uint64_t *prefix = reinterpret_cast<uint64_t *>(factor + ROWS);  // tiles in front of sequence b
-  uint64_t *full = prefix + w.r.batch + 1, *empty = full + STAGES;
-  uint32_t *words = reinterpret_cast<uint32_t *>(empty + STAGES);
+  PagedSeq *seqs = reinterpret_cast<PagedSeq *>(factor + ROWS);
+  uint64_t *prefix = reinterpret_cast<uint64_t *>(seqs + w.r.batch);  // tiles in front of sequence b
+  uint64_t *full = prefix + w.r.batch + 1, *empty = full + STAGES, *qread = empty + STAGES;
+  uint32_t *words = reinterpret_cast<uint32_t *>(qread + 1);
   volatile int *abort_flag = reinterpret_cast<volatile int *>(words);
   const uint32_t tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, (int)tid >> 5, 0);
@@ -121,6 +128,7 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], PM_WARPS);
     }
+    mbar_init(qread, PM_WARPS);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&w.k) : "memory");
@@ -128,12 +136,12 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
   }
   pdl_launch_dependents();
   pdl_wait();
-  // ---- every CTA's share of the tiles
+  // ---- every CTA's share of the tiles: a list of tiles per row block and KV head, PM_LIST places of its own in front of each
   for (uint32_t b = tid; b < w.r.batch; b += PM_THREADS) {
-    const PagedSeq s = paged_seq(w.r, max_len, b);
+    const PagedSeq s = seqs[b] = paged_seq(w.r, max_len, b);
     uint32_t tile0, tiles, blocks;
     seq_tiles(s, group, ROWS, w.window, tile0, tiles, blocks);
-    prefix[b + 1] = (uint64_t)blocks * w.c.kv_heads * tiles;
+    prefix[b + 1] = (uint64_t)blocks * w.c.kv_heads * (tiles + PM_LIST);
   }
   __syncthreads();
   if (warp == 0) {
@@ -155,61 +163,91 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
   uint64_t at = min(total, share * blockIdx.x);
   const uint64_t stop = min(total, at + share);
 
-  // The segment that begins at tile `u` of all; lists are [sequence][block][KV head][tile].
-  auto segment = [&](uint64_t u, Segment &g) {
-    uint32_t lo = 0, hi = w.r.batch;  // prefix[lo] <= u < prefix[hi]
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) / 2;
-      if (prefix[mid] <= u)
-        lo = mid;
-      else
-        hi = mid;
+  // The next segment from place `at` on, false when the share ends; lists are [sequence][block][KV head][list's places].
+  uint32_t cur = 0;
+  auto segment = [&](Segment &g) {
+    while (at < stop) {
+      if (prefix[cur + 1] <= at) {  // rarely further than the next sequence, but at the share's beginning
+        uint32_t lo = cur + 1, hi = w.r.batch;
+        if (prefix[lo + 1] <= at) {  // prefix[lo] <= at < prefix[hi]
+          while (hi - lo > 1) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (prefix[mid] <= at)
+              lo = mid;
+            else
+              hi = mid;
+          }
+        }
+        cur = lo;
+      }
+      g.b = cur;
+      g.s = seqs[cur];
+      uint32_t tile0, tiles, blocks;
+      seq_tiles(g.s, group, ROWS, w.window, tile0, tiles, blocks);
+      const uint32_t places = tiles + PM_LIST;
+      const uint64_t in = at - prefix[cur], item = in >> 32 ? in / places : (uint32_t)in / places;
+      const uint32_t p = (uint32_t)(in - item * places), n = (uint32_t)min((uint64_t)(places - p), stop - at);
+      g.g = (uint32_t)(item % w.c.kv_heads);
+      g.R0 = (uint32_t)(item / w.c.kv_heads) * ROWS;
+      g.R1 = g.s.rows * group;
+      g.begin = at - p + PM_LIST;
+      g.end = g.begin + tiles;
+      at += n;
+      const uint32_t t = max(p, PM_LIST) - PM_LIST, z = max(p + n, PM_LIST) - PM_LIST;
+      if (t == z) continue;
+      g.first = t == 0;
+      g.last = z == tiles;
+      // of these, the tiles that some row of the block sees
+      const int from = w.window ? g.s.pos0 + (int)(g.R0 / group) - (int)w.window + 1 : 0;
+      const int to = g.s.pos0 + (int)((min(g.R1, g.R0 + ROWS) - 1) / group) + 1;  // behind its last row's position
+      const uint32_t k0 = from > 0 ? (uint32_t)from / PM_KEYS : 0, k1 = to > 0 ? ((uint32_t)to + PM_KEYS - 1) / PM_KEYS : 0;
+      g.t0 = max(k0, tile0 + t);
+      g.t1 = max(g.t0, min(k1, tile0 + z));
+      return true;
     }
-    g.b = lo;
-    g.s = paged_seq(w.r, max_len, lo);
-    uint32_t tile0, tiles, blocks;
-    seq_tiles(g.s, group, ROWS, w.window, tile0, tiles, blocks);
-    const uint64_t in = u - prefix[lo], item = in / tiles;
-    const uint32_t t = (uint32_t)(in - item * tiles);
-    g.g = (uint32_t)(item % w.c.kv_heads);
-    g.R0 = (uint32_t)(item / w.c.kv_heads) * ROWS;
-    g.R1 = g.s.rows * group;
-    g.begin = u - t;
-    g.end = g.begin + tiles;
-    const uint32_t n = (uint32_t)min((uint64_t)(tiles - t), stop - u);
-    g.first = t == 0;
-    g.last = t + n == tiles;
-    // of these, the tiles that some row of the block sees
-    const int from = w.window ? g.s.pos0 + (int)(g.R0 / group) - (int)w.window + 1 : 0;
-    const int to = g.s.pos0 + (int)((min(g.R1, g.R0 + ROWS) - 1) / group) + 1;  // behind its last row's position
-    const uint32_t a = from > 0 ? (uint32_t)from / PM_KEYS : 0, z = to > 0 ? ((uint32_t)to + PM_KEYS - 1) / PM_KEYS : 0;
-    g.t0 = max(a, tile0 + t);
-    g.t1 = max(g.t0, min(z, tile0 + t + n));
-    return u + n;
+    return false;
   };
 
   if (warp == PM_WARPS) {
     // ---- pages into the ring.  A tile is 64 / page boxes (or a part of one page) per 64 elements and pool, one lane each.
     const uint32_t box = min(w.c.page, PM_KEYS), boxes = PM_KEYS / box;
-    uint32_t it = 0;
+    uint32_t it = 0, lists = 0;
     bool ok = true;
-    while (at < stop) {
-      Segment g;
-      at = segment(at, g);
-      const int32_t *table = w.c.table + (size_t)g.b * w.c.ld_table;
-      auto page_of = [&](uint32_t t) {
-        const uint32_t p = t * PM_KEYS + lane * box;
-        return lane < boxes && p < g.s.len ? __ldcg(table + p / w.c.page) : -1;
-      };
-      int next = g.t0 < g.t1 ? page_of(g.t0) : -1;
+    Segment g, n;
+    auto page_of = [&](const Segment &x, uint32_t t) {
+      const uint32_t p = t * PM_KEYS + lane * box;
+      return lane < boxes && t < x.t1 && p < x.s.len ? __ldcg(w.c.table + (size_t)x.b * w.c.ld_table + p / w.c.page) : -1;
+    };
+    bool more = segment(n);
+    int next = more ? page_of(n, n.t0) : -1;
+    while (more) {
+      g = n;
+      const uint32_t rows = min(ROWS, g.R1 - g.R0), row_bytes = w.c.dim * (F32 ? 4 : 2);
+      if (g.t0 == g.t1) {
+        if ((more = segment(n))) next = page_of(n, n.t0);
+        continue;
+      }
       for (uint32_t t = g.t0; t < g.t1; ++t, ++it) {
-        const int id = next;
-        if (t + 1 < g.t1) next = page_of(t + 1);
+        const int id = next;  // page ids are asked for a tile ahead
+        if (t + 1 < g.t1)
+          next = page_of(g, t + 1);
+        else if ((more = segment(n)))
+          next = page_of(n, n.t0);
         const uint32_t st = it % STAGES;
-        if (ok) ok = mbar_wait(&empty[st], ((it / STAGES) & 1) ^ 1, abort_flag, 800 + st);
+        if (ok) ok = mbar_wait_now(&empty[st], ((it / STAGES) & 1) ^ 1, abort_flag, 800 + st);
+        const bool queries = MT == 1 && t == g.t0;  // with the block's first tile
+        if (queries) {
+          if (ok) ok = mbar_wait_now(qread, (lists & 1) ^ 1, abort_flag, 805);
+          ++lists;
+        }
         ok = __all_sync(0xffffffffu, ok);
-        if (lane == 0 && ok) mbar_arrive_expect_tx(&full[st], 2 * Z::TILE);
+        if (lane == 0 && ok) mbar_arrive_expect_tx(&full[st], 2 * Z::TILE + (queries ? rows * row_bytes : 0));
         __syncwarp();
+        if (ok && queries && lane < rows) {
+          const uint32_t R = g.R0 + lane;
+          const size_t i = (size_t)(g.s.first + R / group) * w.ld_q + (size_t)(g.g * group + R % group) * w.c.dim;
+          bulk_load(qr + lane * Z::RAW, static_cast<const uint8_t *>(w.q) + i * (F32 ? 4 : 2), row_bytes, &full[st]);
+        }
         if (ok && lane < boxes) {
           const uint32_t p = t * PM_KEYS + lane * box;
           // no page: rows in front of the pool, which read as zeros
@@ -228,9 +266,8 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
     const uint32_t gq = lane >> 2, t4 = lane & 3, mat = lane >> 3, r8 = lane & 7;
     uint32_t it = 0;
     bool ok = true;
-    while (at < stop) {
-      Segment g;
-      at = segment(at, g);
+    Segment g;
+    while (segment(g)) {
       const uint32_t rows = min(ROWS, g.R1 - g.R0);
       // ---- queries: 16 MT rows, absent ones and elements behind dim as zeros
       uint32_t qf[MT == 1 ? DH / 16 : 1][TERMS][4];
@@ -244,14 +281,21 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
       };
       // fp32 rows are divided by the power of two in front of their largest element, whatever it is, so that their terms keep their bits.
       auto down = [&](float most) { return most > 0.f && most < INFINITY ? exp2f(-(float)max(-100, min(100, ilogbf(most)))) : 1.f; };
-      if (MT == 1) {
+      if (MT == 1 && g.t0 < g.t1) {
+        if (ok) ok = mbar_wait_now(&full[it % STAGES], (it / STAGES) & 1, abort_flag, 815);
+        ok = __all_sync(0xffffffffu, ok);
+        auto raw_at = [&](uint32_t r, uint32_t e) -> float2 {
+          if (r >= rows || e >= w.c.dim) return make_float2(0.f, 0.f);
+          if (F32) return *reinterpret_cast<const float2 *>(qr + r * Z::RAW + e * 4);
+          return unpack2<BF16>(*reinterpret_cast<const uint32_t *>(qr + r * Z::RAW + e * 2));
+        };
         float2 x[DH / 16][4];
         float most[2] = {0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < DH / 16; ++ks)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            x[ks][c] = q_at(gq + (c & 1) * 8, ks * 16 + (c >> 1) * 8 + 2 * t4);
+            x[ks][c] = raw_at(gq + (c & 1) * 8, ks * 16 + (c >> 1) * 8 + 2 * t4);
             most[c & 1] = fmaxf(most[c & 1], fmaxf(fabsf(x[ks][c].x), fabsf(x[ks][c].y)));
           }
         float f[2] = {1.f, 1.f};
@@ -274,7 +318,9 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
 #pragma unroll
             for (int i = 0; i < TERMS; ++i) qf[ks][i][c] = v[i];
           }
-      } else {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qread);
+      } else if (MT > 1) {
         bar_math();  // the rows before have been read
         for (uint32_t r = warp; r < ROWS; r += PM_WARPS) {
           float2 x[DH / 64];
@@ -328,7 +374,7 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
       for (uint32_t t = g.t0; t < g.t1; ++t, ++it) {
         const uint32_t st = it % STAGES;
         uint8_t *kt = ring + (size_t)st * 2 * Z::TILE, *vt = kt + Z::TILE;
-        if (ok) ok = mbar_wait(&full[st], (it / STAGES) & 1, abort_flag, 810 + st);
+        if (ok) ok = mbar_wait_now(&full[st], (it / STAGES) & 1, abort_flag, 810 + st);
         ok = __all_sync(0xffffffffu, ok);
         // ---- scores of the warp's 16 keys
         float s[MT][2][4];
@@ -421,7 +467,15 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
           }
         }
         bar_math();
-        // ---- outputs: the warp's DH / 4 elements, 64 keys
+        // ---- outputs: the warp's DH / 4 elements, 64 keys.  The tensor core cuts sums off at the accumulator's last bit: a tile's products meet in
+        // accumulators of their own, added to the row's by an fp32 add that rounds (error of 16 sequences over 4096 keys 4.0e-6 -> see below).
+        float po[MT][DH / 32][4];
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int n = 0; n < (int)DH / 32; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) po[m][n][j] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < 4; ++kk) {
           uint32_t vb[DH / 64][4];
@@ -439,11 +493,17 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
               ldsm_x4(a, ps + (size_t)(i * ROWS + m * 16 + (mat & 1) * 8 + r8) * Z::PP + kk * 32 + (mat >> 1) * 16);
 #pragma unroll
               for (int n = 0; n < (int)DH / 64; ++n) {
-                mma<BF16>(o[m][2 * n], a, vb[n][0], vb[n][1]);
-                mma<BF16>(o[m][2 * n + 1], a, vb[n][2], vb[n][3]);
+                mma<BF16>(po[m][2 * n], a, vb[n][0], vb[n][1]);
+                mma<BF16>(po[m][2 * n + 1], a, vb[n][2], vb[n][3]);
               }
             }
         }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int n = 0; n < (int)DH / 32; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[m][n][j] += po[m][n][j];
         if (k0 + (int)PM_KEYS > end) fence_proxy_async();  // the zeros are in front of the next copy
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
