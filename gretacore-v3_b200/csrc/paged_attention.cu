@@ -530,16 +530,21 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+        for (int c = 0; c < 2; ++c) {
+          const uint32_t r = m * 16 + gq + c * 8;
+          float y[DH / 16], z = 0.f;  // z: 0, or NaN
 #pragma unroll
-          for (int n = 0; n < (int)DH / 32; ++n)
+          for (int n = 0; n < (int)DH / 16; ++n) {
+            y[n] = o[m][n / 2][2 * c + (n & 1)];
+            z = fmaf(y[n], 0.f, z);
+          }
+          if (z != 0.f && r < rows) {
+            paged_again<DH / 16>(w, BF16, F32, g.b, g.s, g.g, g.R0 + r, [&](int n) { return warp * (DH / 4) + n / 2 * 8 + 2 * t4 + (n & 1); },
+                                 max(lim0[m][c], (int)(g.t0 * PM_KEYS)), min(lim1[m][c], (int)(g.t1 * PM_KEYS)), mx[m][c], y);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const uint32_t r = m * 16 + gq + c * 8, e = warp * (DH / 4) + n * 8 + 2 * t4 + j;
-              if (r < rows && e < w.c.dim && !isfinite(o[m][n][2 * c + j]) && g.t0 < g.t1)
-                o[m][n][2 * c + j] = paged_again(w, BF16, F32, g.b, g.s, g.g, g.R0 + r, e, max(lim0[m][c], (int)(g.t0 * PM_KEYS)),
-                                                 min(lim1[m][c], (int)(g.t1 * PM_KEYS)), mx[m][c], o[m][n][2 * c + j]);
-            }
+            for (int n = 0; n < (int)DH / 16; ++n) o[m][n / 2][2 * c + (n & 1)] = y[n];
+          }
+        }
       // ---- a part of the block's tiles: to the workspace, and whoever is last joins the parts
       bool mine = true;
       if (!(g.first && g.last)) {
@@ -688,7 +693,7 @@ int greta_cuda_paged_attn(greta_stream_t stream, const greta_paged_cache *cache,
   GRETA_REQUIRE(aligned16(q) && aligned16(o) && (size_t)ld_q * paged_size(q_fmt) % 16 == 0 && (size_t)ld_o * paged_size(q_fmt) % 16 == 0,
                 "paged_attn: rows that do not begin at 16-byte boundaries");
   GRETA_REQUIRE(q != o, "paged_attn: in place");
-  GRETA_REQUIRE(window < (1u << 31) && isfinite(scale), "paged_attn: window %u, scale %g", window, scale);
+  GRETA_REQUIRE(window < (1u << 31) && scale > 0 && isfinite(scale), "paged_attn: window %u, scale %g", window, scale);
   GRETA_REQUIRE(aligned16(workspace) && workspace_bytes >= greta_cuda_paged_attn_workspace_bytes(d), "paged_attn: workspace of %zu bytes, %zu needed", workspace_bytes,
                 greta_cuda_paged_attn_workspace_bytes(d));
   if (rows->tokens == 0) return GRETA_OK;
@@ -710,11 +715,14 @@ int greta_cuda_paged_attn(greta_stream_t stream, const greta_paged_cache *cache,
   w.tickets = static_cast<uint32_t *>(workspace);
   w.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + PAGED_TICKETS);
   if (int rc = gemm_ts_error_word(&w.error)) return rc;
-  if (int rc = pool_map(&w.k, enc, *cache, cache->k, std::min(cache->page, PM_KEYS))) return rc;
-  if (int rc = pool_map(&w.v, enc, *cache, cache->v, std::min(cache->page, PM_KEYS))) return rc;
   const uint32_t most = rows->max_rows ? std::min(rows->max_rows, rows->tokens) : rows->tokens;
   const bool many = (uint64_t)most * w.group > 16, bf16 = cache->fmt == GRETA_FMT_BF16, f32 = q_fmt == GRETA_FMT_F32;
+  const bool tc = many && !f32 && w.group <= 128;
+  const uint32_t box = std::min(cache->page, tc ? 128 : PM_KEYS);
+  if (int rc = pool_map(&w.k, enc, *cache, cache->k, box)) return rc;
+  if (int rc = pool_map(&w.v, enc, *cache, cache->v, box)) return rc;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (tc) return paged_attn_tc(s, w, heads);
   if (d > 64) return bf16 ? launch_mma<2, true>(s, w, f32, many) : launch_mma<2, false>(s, w, f32, many);
   return bf16 ? launch_mma<1, true>(s, w, f32, many) : launch_mma<1, false>(s, w, f32, many);
 }

@@ -10,6 +10,7 @@ int gemm_ts_error_word(int **word);  // gemm_ts.cu: the word that greta_cuda_gem
 
 struct PagedAttnArgs {
   CUtensorMap k, v;  // the pools as rows of `dim` elements; rows outside read as zeros
+  CUtensorMap qm;    // queries of 16 bits
   greta_paged_cache c;
   greta_ragged r;
   const void *q;
@@ -25,34 +26,42 @@ constexpr uint32_t PAGED_CTAS_PER_SM = 2, PAGED_MAX_CTAS = 512;
 constexpr uint32_t PAGED_TICKETS = 65536;  // bytes
 constexpr uint32_t PAGED_PART = 64 * (128 + 2);
 
+int paged_attn_tc(cudaStream_t stream, PagedAttnArgs &w, uint32_t heads);  // paged_attention_tc.cu
+
 #ifdef __CUDACC__
-// Element e of row R's unnormalised output over keys k0 .. k1 - 1 (all seen by the row), whose maximum is mx: taken again where the product with
-// hidden keys' values left no finite number.  `was` stays if a value that the row sees is none either.  Rare and slow: a key at a time.
-__device__ __noinline__ float paged_again(const PagedAttnArgs &w, bool bf16, bool f32, uint32_t b, const PagedSeq &s, uint32_t g, uint32_t R, uint32_t e, int k0, int k1,
-                                          float mx, float was) {
+// Elements elem(0 .. N - 1) of row R's unnormalised output over the keys k0 .. k1 - 1 (all seen by the row), whose scores are taken against mx: again, where the
+// product with hidden keys' values left no finite numbers.  An element stays as it was if a value that the row sees is none either.  Rare and slow: a key at a time.
+template <int N, typename Elem>
+__device__ __noinline__ void paged_again(const PagedAttnArgs &w, bool bf16, bool f32, uint32_t b, const PagedSeq &s, uint32_t g, uint32_t R, Elem elem, int k0, int k1, float mx,
+                                         float (&y)[N]) {
   const uint32_t d = w.c.dim;
   const int32_t *table = w.c.table + (size_t)b * w.c.ld_table;
   auto value = [&](const void *p, size_t i) {
     const uint16_t x = static_cast<const uint16_t *>(p)[i];
     return bf16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
   };
-  auto row_of = [&](int j, size_t &row) {
-    const int id = table[(uint32_t)j / w.c.page];
-    row = (((size_t)id * w.c.kv_heads + g) * w.c.page + (uint32_t)j % w.c.page) * d;
-    return id >= 0 && (uint32_t)id < w.c.pages;
-  };
-  size_t row;
-  for (int j = k0; j < k1; ++j)
-    if (row_of(j, row) && !isfinite(value(w.c.v, row + e))) return was;
+  uint32_t again = 0;
+  for (int n = 0; n < N; ++n)
+    if (elem(n) < d && !isfinite(y[n])) again |= 1u << n;
   const size_t qi = (size_t)(s.first + R / w.group) * w.ld_q + (size_t)(g * w.group + R % w.group) * d;
-  float acc = 0.f;
-  for (int j = k0; j < k1; ++j) {
-    if (!row_of(j, row)) continue;  // a value of zero
+  float acc[N];
+  for (int n = 0; n < N; ++n) acc[n] = 0.f;
+  for (int j = k0; j < k1 && again; ++j) {
+    const int id = table[(uint32_t)j / w.c.page];
+    if (id < 0 || (uint32_t)id >= w.c.pages) continue;  // a value of zero
+    const size_t row = (((size_t)id * w.c.kv_heads + g) * w.c.page + (uint32_t)j % w.c.page) * d;
     float t = 0.f;
     for (uint32_t i = 0; i < d; ++i) t = fmaf(f32 ? static_cast<const float *>(w.q)[qi + i] : value(w.q, qi + i), value(w.c.k, row + i), t);
-    acc = fmaf(exp2f(t * w.scale2 - mx), value(w.c.v, row + e), acc);
+    const float p = exp2f(t * w.scale2 - mx);
+    for (int n = 0; n < N; ++n)
+      if (again >> n & 1) {
+        const float x = value(w.c.v, row + elem(n));
+        if (!isfinite(x)) again &= ~(1u << n);
+        acc[n] = fmaf(p, x, acc[n]);
+      }
   }
-  return acc;
+  for (int n = 0; n < N; ++n)
+    if (again >> n & 1) y[n] = acc[n];
 }
 #endif
 
