@@ -3,8 +3,8 @@
 // A CTA takes a block of 256 query rows of one KV head as two tiles of 128: row R of a sequence and KV head is token R / group, head R % group, so a tile
 // is 128 / group tokens with all their heads and every key tile is fetched once for them.  Keys come in tiles of 128, page by page, by TMA (a page's rows of a head
 // are contiguous); queries by TMA as boxes of [tokens][group][64].
-//   warp 0: copies; warp 1: MMAs; warp 2: zeros over what a page holds behind the sequence's end; warps 4-7 and 8-11: a query row per thread of the first
-//   and second tile: maxima, probabilities, outputs.
+//   warp 0: copies, and zeros over what the last page holds behind the sequence's end; warp 1: MMAs; warps 2-5 and 6-9: a query row per thread of the
+//   first and second tile: maxima, probabilities, outputs.
 // The two tiles take turns: while the tensor core multiplies one (P V of this key tile, Q K of the next), the other's probabilities are made.
 //   tensor memory: scores of tile A and B at columns 0 and 128, each overwritten by its probabilities (64 columns), outputs at 256 and 384.
 // A row's sums are rescaled only when its maximum has grown by more than 2^8 (probabilities up to 2^8 fit every type); the scores' barrier of a key tile says that
@@ -21,8 +21,9 @@ using namespace greta;
 
 namespace {
 
-constexpr uint32_t PT_ROWS = 128, PT_KEYS = 128, PT_THREADS = 384, PT_UNITS = 5, PT_TMEM = 512;
+constexpr uint32_t PT_ROWS = 128, PT_KEYS = 128, PT_THREADS = 320, PT_UNITS = 5, PT_TMEM = 512;
 constexpr uint32_t PT_SLAB = 128 * 128;  // bytes of 64 elements of 128 rows
+constexpr int PT_EMULATED = 1;           // pairs of probabilities out of four that the FMA units make: the special-function unit's 16 a clock bound the tile otherwise
 constexpr float PT_LAZY = 8.f;           // log2 of what a row's maximum may grow by before its sums are rescaled
 constexpr float PT_LOWEST = -3.4028234e38f;  // a row's maximum before any score
 
@@ -43,6 +44,41 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of two values without the special-function unit: x = n + r, n an integer (by adding 1.5 * 2^23, whose last place is one) and |r| <= 1/2; a polynomial in r of
+// degree 3, fitted to the smallest largest relative error over that interval (7.5e-5, a quarter of half a step of fp16); n is added to its exponent.
+__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
+  const uint64_t big = pair(12582912.f, 12582912.f);
+  const float2 f = unpair(x);
+  x = pair(fmaxf(f.x, -126.f), fmaxf(f.y, -126.f));
+  const uint64_t t = add2(x, big), n = add2(t, pair(-12582912.f, -12582912.f)), r = fma2(n, pair(-1.f, -1.f), x);
+  uint64_t p = fma2(r, pair(0.0551716685f, 0.0551716685f), pair(0.242611125f, 0.242611125f));
+  p = fma2(p, r, pair(0.693260968f, 0.693260968f));
+  p = fma2(p, r, pair(0.999928057f, 0.999928057f));
+  const float2 y = unpair(p), e = unpair(t);
+  return pair(__int_as_float(__float_as_int(y.x) + (__float_as_int(e.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(e.y) << 23)));
+}
+
 // A block of rows of one sequence and KV head, and the key tiles of its two halves.
 struct Block {
   uint32_t b, g, token0, t0, t1;      // tiles t0 .. t1 - 1 of either half
@@ -57,7 +93,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
   uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t *qs = smem, *ring = qs + 2 * UNIT;  // queries of both tiles; keys and values in turn
   uint64_t *bars = reinterpret_cast<uint64_t *>(ring + PT_UNITS * UNIT);
-  uint64_t *full = bars, *empty = full + PT_UNITS, *qf = empty + PT_UNITS, *sf = qf + 1, *pf = sf + 2, *vl = pf + 2, *vz = vl + 1, *fin = vz + 1;  // vl: the last values have come; vz: and hold zeros behind the sequence
+  uint64_t *full = bars, *empty = full + PT_UNITS, *qf = empty + PT_UNITS, *sf = qf + 1, *pf = sf + 2, *vl = pf + 4, *vz = vl + 1, *fin = vz + 1;  // vl: the last values have come; vz: and hold zeros behind the sequence
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(fin + 2), *place = tmem_slot + 1;  // place: sequence, block
   volatile int *abort_flag = reinterpret_cast<volatile int *>(place + 2);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -73,7 +109,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     mbar_init(vz, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sf[i], 1);
-      mbar_init(&pf[i], 4);
+      mbar_init(&pf[2 * i], 4);  // probabilities of a tile's first and second 64 keys
+      mbar_init(&pf[2 * i + 1], 4);
       mbar_init(&fin[i], 1);
     }
     place[0] = 0xffffffffu;
@@ -96,7 +133,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 
   // ---- which block: sequences in order, the last rows of each (the longest) first, KV heads side by side
   const uint32_t max_len = w.c.ld_table * w.c.page, heads_kv = w.c.kv_heads;
-  if (warp == 3) {
+  if (warp == 0) {
     uint32_t before = 0;
     const uint32_t mine = blockIdx.x / heads_kv;
     for (uint32_t b0 = 0; b0 < w.r.batch; b0 += 32) {
@@ -172,6 +209,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             for (uint32_t c = 0; c < SD; ++c) tma_load_2d(ring + st * UNIT + c * PT_SLAB + lane * box * 128, kv ? &w.v : &w.k, (int)(c * 64), row, bar);
         }
       }
+      if (ragged) {  // what the last page holds behind the sequence's end: zeros
+        if (ok) ok = mbar_wait(vl, 0, abort_flag, 950);
+        __syncwarp();
+        const uint32_t from = (uint32_t)max(0, last - (int)((k.t1 - 1) * PT_KEYS));
+        if (ok) {
+          for (uint32_t i = lane; i < (PT_KEYS - from) * 8 * SD; i += 32)
+            *reinterpret_cast<uint4 *>(ring + (it - 1) % PT_UNITS * UNIT + i / ((PT_KEYS - from) * 8) * PT_SLAB + from * 128 + i % ((PT_KEYS - from) * 8) * 16) =
+                make_uint4(0, 0, 0, 0);
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (leader && ok) mbar_arrive(vz);
+      }
       if (leader && *abort_flag) drain_copies(full, it, PT_UNITS);
       if (leader && *abort_flag) drain_copies(qf, 1, 1);
       if (leader && *abort_flag) drain_copies(vl, ragged ? 1 : 0, 1);
@@ -207,14 +257,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
               if (ok) ok = ragged && t == k.t1 ? poll(vz, 0, abort_flag, 921) : poll(&full[iv % PT_UNITS], (iv / PT_UNITS) & 1, abort_flag, 920);
               have_v = true;
             }
-            if (ok) ok = poll(&pf[i], np[i] & 1, abort_flag, 930 + i);
-            __syncwarp();
-            if (leader && ok) {
-              tc_fence_after();
 #pragma unroll
-              for (uint32_t k16 = 0; k16 < PT_KEYS / 16; ++k16)
-                umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + k16 * 8, v_lo + (iv % PT_UNITS) * (UNIT / 16) + k16 * (2048 >> 4), SMEM_DESC_HI_SW128, idesc_o,
-                            (np[i] | k16) ? 1u : 0u);
+            for (uint32_t part = 0; part < 2; ++part) {
+              if (ok) ok = poll(&pf[2 * i + part], np[i] & 1, abort_flag, 930 + 2 * i + part);
+              __syncwarp();
+              if (leader && ok) {
+                tc_fence_after();
+#pragma unroll
+                for (uint32_t k16 = part * 4; k16 < part * 4 + 4; ++k16) {
+                  umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + k16 * 8, v_lo + (iv % PT_UNITS) * (UNIT / 16) + k16 * (2048 >> 4), SMEM_DESC_HI_SW128, idesc_o,
+                              (np[i] | k16) ? 1u : 0u);
+                }
+              }
+            }
+            if (leader && ok) {
               if (t == k.hi[i]) umma_commit(&fin[i]);
             }
             ++np[i];
@@ -232,20 +288,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         if (leader && ok && vt) umma_commit(&empty[iv % PT_UNITS]);
         if (leader && ok && kt) umma_commit(&empty[ik % PT_UNITS]);
       }
-    } else if (warp == 2) {
-      if (ragged) {
-        const uint32_t iv = 2 * (k.t1 - 1 - k.t0) + 1, st = iv % PT_UNITS;
-        const bool ok = mbar_wait_warp(vl, 0, abort_flag, 950);
-        const uint32_t from = (uint32_t)max(0, last - (int)((k.t1 - 1) * PT_KEYS));
-        if (ok)
-          for (uint32_t i = lane; i < (PT_KEYS - from) * 8 * SD; i += 32)
-            *reinterpret_cast<uint4 *>(ring + st * UNIT + i / ((PT_KEYS - from) * 8) * PT_SLAB + from * 128 + i % ((PT_KEYS - from) * 8) * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0 && ok) mbar_arrive(vz);
-      }
-    } else if (warp >= 4) {
-      const uint32_t i = warp >= 8 ? 1 : 0, quad = warp & 3, row = quad * 32 + lane;
+    } else {
+      const uint32_t i = warp >= 6 ? 1 : 0, quad = warp & 3, row = quad * 32 + lane;
       const uint32_t lanes = tmem + (quad * 32 << 16), sb = lanes + i * 128, ob = lanes + 256 + i * 128;
       const bool live = row < k.tokens[i] * group;
       const uint32_t token = k.token0 + i * TT + row / group;
@@ -254,6 +298,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
       // tiles that every live row of the half sees whole need no masks
       const int pos_lo = k.s.pos0 + (int)(k.token0 + i * TT), pos_hi = pos_lo + (int)k.tokens[i] - 1;
       const int whole0 = w.window ? max(0, pos_hi - (int)w.window + 1) : 0, whole1 = pos_lo + 1;
+      const bool any_live = quad * 32 < k.tokens[i] * group;
       float m2 = PT_LOWEST, l = 0.f;  // the row's maximum times scale2
       bool ok = true;
       uint32_t n = 0;
@@ -261,23 +306,41 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         ok = __all_sync(0xffffffffu, poll(&sf[i], n & 1, abort_flag, 960 + i));
         if (!ok) break;
         tc_fence_after();
-        uint32_t v[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(sb + c * 32, v[c]);
-        tmem_ld_wait();
-        const int k0 = (int)(t * PT_KEYS);
-        if (k0 < whole0 || k0 + (int)PT_KEYS > whole1) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (k0 + c * 32 + j < lim0 || k0 + c * 32 + j >= lim1) v[c][j] = 0xFF800000u;
+        if (!any_live) {  // rows behind the last: their probabilities may be anything
+          if (lane == 0) {
+            mbar_arrive(&pf[2 * i]);
+            mbar_arrive(&pf[2 * i + 1]);
+          }
+          continue;
         }
+        uint32_t v[4][32];
+        const int k0 = (int)(t * PT_KEYS);
+        const bool masks = k0 < whole0 || k0 + (int)PT_KEYS > whole1;
         float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        tmem_ld32(sb, v[0]);
+        tmem_ld32(sb + 32, v[1]);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int h = 0; h < 2; ++h) {
+          tmem_ld_wait();
+          if (h == 0) {
+            tmem_ld32(sb + 64, v[2]);
+            tmem_ld32(sb + 96, v[3]);
+          }
 #pragma unroll
-          for (int j = 0; j < 32; ++j) tm[j & 3] = fmaxf(tm[j & 3], __uint_as_float(v[c][j]));
+          for (int c = 2 * h; c < 2 * h + 2; ++c) {
+            if (masks) {
+              const int n0 = min(max(lim0 - k0 - c * 32, 0), 32), n1 = min(max(lim1 - k0 - c * 32, 0), 32);
+              const uint32_t seen = (uint32_t)((1ull << n1) - 1) & ~(uint32_t)((1ull << n0) - 1);
+              if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                  if (!(seen >> j & 1)) v[c][j] = 0xFF800000u;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) tm[(j / 2) & 3] = fmaxf(fmaxf(tm[(j / 2) & 3], __uint_as_float(v[c][j])), __uint_as_float(v[c][j + 1]));
+          }
+        }
         const float nm = fmaxf(m2, fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3])) * w.scale2);
         if (n == 0) {
           m2 = nm;
@@ -286,38 +349,53 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
           if (nm > m2 + PT_LAZY) m2 = nm;
           l *= f;
 #pragma unroll 1
-          for (uint32_t c = 0; c < DH; c += 32) {
-            uint32_t o[32];
-            tmem_ld32(ob + c, o);
+          for (uint32_t c = 0; c < DH; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(ob + c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-            tmem_st32(ob + c, o);
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+            tmem_st16(ob + c, o);
           }
         }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint64_t sum[2] = {0, 0};
+        const uint64_t scale = pair(w.scale2, w.scale2), minus = pair(-m2, -m2);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t p[32];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t p[16];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float p0 = ex2(fmaf(__uint_as_float(v[2 * c + j / 16][(2 * j) & 31]), w.scale2, -m2)), p1 = ex2(fmaf(__uint_as_float(v[2 * c + j / 16][(2 * j + 1) & 31]), w.scale2, -m2));
-            sum[(2 * j) & 3] += p0;
-            sum[(2 * j + 1) & 3] += p1;
-            p[j] = pack2<BF16>(p0, p1);
+          for (int j = 0; j < 16; ++j) {
+            uint64_t x = fma2(pair(__uint_as_float(v[c][2 * j]), __uint_as_float(v[c][2 * j + 1])), scale, minus);
+            if ((j & 3) < PT_EMULATED) {
+              x = exp2_pair(x);
+            } else {
+              const float2 f = unpair(x);
+              x = pair(ex2(f.x), ex2(f.y));
+            }
+            sum[j & 1] = add2(sum[j & 1], x);
+            const float2 f = unpair(x);
+            p[j] = pack2<BF16>(f.x, f.y);
           }
-          tmem_st32(sb + c * 32, p);
+          // The products of the first 64 keys begin while the other probabilities are made.
+          if (c == 2) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pf[2 * i]);
+          }
+          tmem_st16(sb + c * 16, p);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        const float2 s0 = unpair(sum[0]), s1 = unpair(sum[1]);
+        l += (s0.x + s0.y) + (s1.x + s1.y);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&pf[i]);
+        if (lane == 0) mbar_arrive(&pf[2 * i + 1]);
       }
       if (ok && n) ok = __all_sync(0xffffffffu, poll(&fin[i], 0, abort_flag, 970 + i));
       if (ok && k.tokens[i]) {
         tc_fence_after();
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const float inv = m2 == PT_LOWEST ? 0.f : 1.f / l;  // a row that has seen no score: zeros (its sum holds what 2^-126 is for minus infinity)
         uint16_t *out = static_cast<uint16_t *>(w.o) + (size_t)(k.s.first + token) * w.ld_o + (size_t)(k.g * group + row % group) * w.c.dim;
 #pragma unroll 1
         for (uint32_t c = 0; c < DH; c += 32) {
@@ -356,7 +434,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 
 template <int SD, bool BF16>
 int launch_tc(cudaStream_t stream, const PagedAttnArgs &w, uint32_t blocks) {
-  constexpr size_t smem = (size_t)(2 + PT_UNITS) * SD * PT_SLAB + 1024 + (2 * PT_UNITS + 9) * 8 + 16;
+  constexpr size_t smem = (size_t)(2 + PT_UNITS) * SD * PT_SLAB + 1024 + (2 * PT_UNITS + 11) * 8 + 16;
   static bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
