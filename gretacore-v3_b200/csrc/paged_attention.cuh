@@ -30,7 +30,8 @@ int paged_attn_tc(cudaStream_t stream, PagedAttnArgs &w, uint32_t heads);  // pa
 
 #ifdef __CUDACC__
 // Elements elem(0 .. N - 1) of row R's unnormalised output over the keys k0 .. k1 - 1 (all seen by the row), whose scores are taken against mx: again, where the
-// product with hidden keys' values left no finite numbers.  An element stays as it was if a value that the row sees is none either.  Rare and slow: a key at a time.
+// product with hidden keys' values left no finite numbers.  An element stays as it was if a value that the row sees is none either.  Rare and slow: a key at a time, by one
+// thread.  Not for rows whose sum of weights is no finite number: their outputs are none whatever the values are.
 template <int N, typename Elem>
 __device__ __noinline__ void paged_again(const PagedAttnArgs &w, bool bf16, bool f32, uint32_t b, const PagedSeq &s, uint32_t g, uint32_t R, Elem elem, int k0, int k1, float mx,
                                          float (&y)[N]) {
@@ -41,25 +42,37 @@ __device__ __noinline__ void paged_again(const PagedAttnArgs &w, bool bf16, bool
     return bf16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
   };
   uint32_t again = 0;
+#pragma unroll
   for (int n = 0; n < N; ++n)
     if (elem(n) < d && !isfinite(y[n])) again |= 1u << n;
+  auto row_of = [&](int j, size_t &row) {  // false: no page, values of zero
+    const int id = table[(uint32_t)j / w.c.page];
+    row = (((size_t)id * w.c.kv_heads + g) * w.c.page + (uint32_t)j % w.c.page) * d;
+    return id >= 0 && (uint32_t)id < w.c.pages;
+  };
+  size_t row;
+  for (int j = k0; j < k1 && again; ++j) {
+    if (!row_of(j, row)) continue;
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (again >> n & 1 && !isfinite(value(w.c.v, row + elem(n)))) again &= ~(1u << n);
+  }
+  if (!again) return;
   const size_t qi = (size_t)(s.first + R / w.group) * w.ld_q + (size_t)(g * w.group + R % w.group) * d;
   float acc[N];
+#pragma unroll
   for (int n = 0; n < N; ++n) acc[n] = 0.f;
-  for (int j = k0; j < k1 && again; ++j) {
-    const int id = table[(uint32_t)j / w.c.page];
-    if (id < 0 || (uint32_t)id >= w.c.pages) continue;  // a value of zero
-    const size_t row = (((size_t)id * w.c.kv_heads + g) * w.c.page + (uint32_t)j % w.c.page) * d;
+  for (int j = k0; j < k1; ++j) {
+    if (!row_of(j, row)) continue;
     float t = 0.f;
+#pragma unroll 8
     for (uint32_t i = 0; i < d; ++i) t = fmaf(f32 ? static_cast<const float *>(w.q)[qi + i] : value(w.q, qi + i), value(w.c.k, row + i), t);
     const float p = exp2f(t * w.scale2 - mx);
+#pragma unroll
     for (int n = 0; n < N; ++n)
-      if (again >> n & 1) {
-        const float x = value(w.c.v, row + elem(n));
-        if (!isfinite(x)) again &= ~(1u << n);
-        acc[n] = fmaf(p, x, acc[n]);
-      }
+      if (again >> n & 1) acc[n] = fmaf(p, value(w.c.v, row + elem(n)), acc[n]);
   }
+#pragma unroll
   for (int n = 0; n < N; ++n)
     if (again >> n & 1) y[n] = acc[n];
 }

@@ -3,10 +3,10 @@
 // A CTA takes a block of 256 query rows of one KV head as two tiles of 128: row R of a sequence and KV head is token R / group, head R % group, so a tile
 // is 128 / group tokens with all their heads and every key tile is fetched once for them.  Keys come in tiles of 128, page by page, by TMA (a page's rows of a head
 // are contiguous); queries by TMA as boxes of [tokens][group][64].
-//   warp 0: copies, and zeros over what the last page holds behind the sequence's end; warp 1: MMAs; warps 2-5 and 6-9: a query row per thread of the
-//   first and second tile: maxima, probabilities, outputs.
+//   warp 0: copies, and zeros over what the last page holds behind the sequence's end; warp 1: MMAs; warps 2-9 and 10-17: the rows of the first and
+//   second tile, two threads each (64 keys of a tile, half of the outputs): maxima, probabilities, outputs.
 // The two tiles take turns: while the tensor core multiplies one (P V of this key tile, Q K of the next), the other's probabilities are made.
-//   tensor memory: scores of tile A and B at columns 0 and 128, each overwritten by its probabilities (64 columns), outputs at 256 and 384.
+//   tensor memory: scores of tile A and B at columns 0 and 128, each half of which is overwritten by its probabilities (32 columns), outputs at 256 and 384.
 // A row's sums are rescaled only when its maximum has grown by more than 2^8 (probabilities up to 2^8 fit every type); the scores' barrier of a key tile says that
 // the products of the one before are in, so the rows' own threads do that.
 #include <math.h>
@@ -21,7 +21,7 @@ using namespace greta;
 
 namespace {
 
-constexpr uint32_t PT_ROWS = 128, PT_KEYS = 128, PT_THREADS = 320, PT_UNITS = 5, PT_TMEM = 512;
+constexpr uint32_t PT_ROWS = 128, PT_KEYS = 128, PT_THREADS = 576, PT_UNITS = 5, PT_TMEM = 512;
 constexpr uint32_t PT_SLAB = 128 * 128;  // bytes of 64 elements of 128 rows
 constexpr int PT_EMULATED = 1;           // pairs of probabilities out of four that the FMA units make: the special-function unit's 16 a clock bound the tile otherwise
 constexpr float PT_LAZY = 8.f;           // log2 of what a row's maximum may grow by before its sums are rescaled
@@ -32,10 +32,29 @@ __device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *m
                "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
                : "memory");
 }
-// On the critical path: polls (a wait with a time hint wakes late).
+// On the critical path: waits that the hardware ends (a time hint wakes late; testing without rest takes issue slots from the warps that compute).
+__device__ __noinline__ bool poll_slow(uint32_t bar, uint32_t parity, volatile int *abort_flag, int code) {
+  const long long t0 = clock64();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if (*abort_flag) return false;
+    if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
+      *abort_flag = code;
+      return false;
+    }
+  }
+}
 __device__ __forceinline__ bool poll(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int code) {
   if (mbar_try_wait(bar, parity)) return true;
-  return mbar_wait_slow<false>(smem_u32(bar), parity, abort_flag, code);
+  return poll_slow(smem_u32(bar), parity, abort_flag, code);
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -89,12 +108,13 @@ struct Block {
 template <int SD, bool BF16>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttnArgs w) {
   constexpr uint32_t DH = SD * 64, UNIT = SD * PT_SLAB;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) uint8_t paged_tc_smem[];  // alignment of the swizzled tiles; there is no room to align it by hand
+  uint8_t *smem = paged_tc_smem;
   uint8_t *qs = smem, *ring = qs + 2 * UNIT;  // queries of both tiles; keys and values in turn
   uint64_t *bars = reinterpret_cast<uint64_t *>(ring + PT_UNITS * UNIT);
   uint64_t *full = bars, *empty = full + PT_UNITS, *qf = empty + PT_UNITS, *sf = qf + 1, *pf = sf + 2, *vl = pf + 4, *vz = vl + 1, *fin = vz + 1;  // vl: the last values have come; vz: and hold zeros behind the sequence
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(fin + 2), *place = tmem_slot + 1;  // place: sequence, block
+  float *meet = reinterpret_cast<float *>(fin + 2);  // [tile][half][row]: what the two threads of a row tell each other
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(meet + 4 * PT_ROWS), *place = tmem_slot + 1;  // place: sequence, block
   volatile int *abort_flag = reinterpret_cast<volatile int *>(place + 2);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t group = w.group, TT = PT_ROWS / group;
@@ -109,12 +129,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     mbar_init(vz, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&sf[i], 1);
-      mbar_init(&pf[2 * i], 4);  // probabilities of a tile's first and second 64 keys
-      mbar_init(&pf[2 * i + 1], 4);
+      mbar_init(&pf[2 * i], 8);  // the first and the second 32 keys of both warps of a row
+      mbar_init(&pf[2 * i + 1], 8);
       mbar_init(&fin[i], 1);
     }
     place[0] = 0xffffffffu;
-    *abort_flag = 0;
+    *abort_flag = smem_u32(smem) % 1024 ? 999 : 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&w.k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&w.v) : "memory");
@@ -133,7 +153,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 
   // ---- which block: sequences in order, the last rows of each (the longest) first, KV heads side by side
   const uint32_t max_len = w.c.ld_table * w.c.page, heads_kv = w.c.kv_heads;
-  if (warp == 0) {
+  if (warp == 0 && *abort_flag == 0) {
     uint32_t before = 0;
     const uint32_t mine = blockIdx.x / heads_kv;
     for (uint32_t b0 = 0; b0 < w.r.batch; b0 += 32) {
@@ -200,7 +220,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
         for (uint32_t kv = 0; kv < 2; ++kv, ++it) {
           const uint32_t st = it % PT_UNITS;
-          if (ok) ok = mbar_wait(&empty[st], ((it / PT_UNITS) & 1) ^ 1, abort_flag, 900 + st);
+          if (ok) ok = poll(&empty[st], ((it / PT_UNITS) & 1) ^ 1, abort_flag, 900 + st);
           __syncwarp();
           uint64_t *bar = kv && ragged && t + 1 == k.t1 ? vl : &full[st];
           if (leader && ok) mbar_arrive_expect_tx(bar, UNIT);
@@ -264,9 +284,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
               if (leader && ok) {
                 tc_fence_after();
 #pragma unroll
-                for (uint32_t k16 = part * 4; k16 < part * 4 + 4; ++k16) {
-                  umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + k16 * 8, v_lo + (iv % PT_UNITS) * (UNIT / 16) + k16 * (2048 >> 4), SMEM_DESC_HI_SW128, idesc_o,
-                              (np[i] | k16) ? 1u : 0u);
+                for (uint32_t x = 0; x < 4; ++x) {
+                  const uint32_t k16 = (x >> 1) * 4 + part * 2 + (x & 1);  // a half's probabilities lie in the first 32 of its own 64 columns of scores
+                  umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + (x >> 1) * 64 + (part * 2 + (x & 1)) * 8, v_lo + (iv % PT_UNITS) * (UNIT / 16) + k16 * (2048 >> 4),
+                              SMEM_DESC_HI_SW128, idesc_o, (np[i] | part | x) ? 1u : 0u);
                 }
               }
             }
@@ -289,22 +310,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         if (leader && ok && kt) umma_commit(&empty[ik % PT_UNITS]);
       }
     } else {
-      const uint32_t i = warp >= 6 ? 1 : 0, quad = warp & 3, row = quad * 32 + lane;
-      const uint32_t lanes = tmem + (quad * 32 << 16), sb = lanes + i * 128, ob = lanes + 256 + i * 128;
-      const bool live = row < k.tokens[i] * group;
+      const uint32_t i = (uint32_t)(warp - 2) >> 3, half = ((uint32_t)(warp - 2) >> 2) & 1, quad = warp & 3, row = quad * 32 + lane;
+      const uint32_t lanes = tmem + (quad * 32 << 16), sb = lanes + i * 128 + half * 64, ob = lanes + 256 + i * 128 + half * (DH / 2);
+      float *mine = meet + (i * 2 + half) * PT_ROWS + row, *theirs = meet + (i * 2 + (half ^ 1)) * PT_ROWS + row;
+      auto meet_other = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + i * 4 + quad) : "memory"); };  // with the other warp of these rows
+      auto agree = [&](bool x) {  // whether any thread of the two warps says so
+        uint32_t any;
+        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"(1 + i * 4 + quad), "r"((uint32_t)x) : "memory");
+        return any != 0;
+      };
+      const bool live = row < k.tokens[i] * group, any_live = quad * 32 < k.tokens[i] * group;
       const uint32_t token = k.token0 + i * TT + row / group;
       const int pos = k.s.pos0 + (int)token;
       const int lim1 = live ? pos + 1 : 0, lim0 = w.window && pos >= (int)w.window ? pos - (int)w.window + 1 : 0;
-      // tiles that every live row of the half sees whole need no masks
+      // tiles that every live row sees whole need no masks
       const int pos_lo = k.s.pos0 + (int)(k.token0 + i * TT), pos_hi = pos_lo + (int)k.tokens[i] - 1;
       const int whole0 = w.window ? max(0, pos_hi - (int)w.window + 1) : 0, whole1 = pos_lo + 1;
-      const bool any_live = quad * 32 < k.tokens[i] * group;
-      float m2 = PT_LOWEST, l = 0.f;  // the row's maximum times scale2
+      float m2 = PT_LOWEST, l = 0.f;  // the row's maximum times scale2; the sum of this thread's half
       bool ok = true;
       uint32_t n = 0;
-      for (uint32_t t = k.lo[i]; t < k.hi[i] && ok; ++t, ++n) {
-        ok = __all_sync(0xffffffffu, poll(&sf[i], n & 1, abort_flag, 960 + i));
-        if (!ok) break;
+      for (uint32_t t = k.lo[i]; t < k.hi[i]; ++t, ++n) {  // to the end, whatever became of a wait: the two warps of a row meet in every tile
+        if (ok) ok = __all_sync(0xffffffffu, poll(&sf[i], n & 1, abort_flag, 960 + i));
         tc_fence_after();
         if (!any_live) {  // rows behind the last: their probabilities may be anything
           if (lane == 0) {
@@ -313,56 +339,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
           }
           continue;
         }
-        uint32_t v[4][32];
         const int k0 = (int)(t * PT_KEYS);
         const bool masks = k0 < whole0 || k0 + (int)PT_KEYS > whole1;
-        float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        tmem_ld32(sb, v[0]);
-        tmem_ld32(sb + 32, v[1]);
+        uint32_t v[2][32];
+        auto hide = [&](int c) {  // scores of keys that the row does not see
+          if (masks) {
+            const int a = k0 + (int)half * 64 + c * 32, n0 = min(max(lim0 - a, 0), 32), n1 = min(max(lim1 - a, 0), 32);
+            const uint32_t seen = (uint32_t)((1ull << n1) - 1) & ~(uint32_t)((1ull << n0) - 1);
+            if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          tmem_ld_wait();
-          if (h == 0) {
-            tmem_ld32(sb + 64, v[2]);
-            tmem_ld32(sb + 96, v[3]);
-          }
-#pragma unroll
-          for (int c = 2 * h; c < 2 * h + 2; ++c) {
-            if (masks) {
-              const int n0 = min(max(lim0 - k0 - c * 32, 0), 32), n1 = min(max(lim1 - k0 - c * 32, 0), 32);
-              const uint32_t seen = (uint32_t)((1ull << n1) - 1) & ~(uint32_t)((1ull << n0) - 1);
-              if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (!(seen >> j & 1)) v[c][j] = 0xFF800000u;
-              }
+              for (int j = 0; j < 32; ++j)
+                if (!(seen >> j & 1)) v[c][j] = 0xFF800000u;
             }
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) tm[(j / 2) & 3] = fmaxf(fmaxf(tm[(j / 2) & 3], __uint_as_float(v[c][j])), __uint_as_float(v[c][j + 1]));
           }
-        }
-        const float nm = fmaxf(m2, fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3])) * w.scale2);
-        if (n == 0) {
-          m2 = nm;
-        } else if (__any_sync(0xffffffffu, nm > m2 + PT_LAZY)) {
-          const float f = nm > m2 + PT_LAZY ? ex2(m2 - nm) : 1.f;
-          if (nm > m2 + PT_LAZY) m2 = nm;
-          l *= f;
-#pragma unroll 1
-          for (uint32_t c = 0; c < DH; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(ob + c, o);
-            tmem_ld_wait();
+        };
+        auto largest = [&](int c) {
+          float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-            tmem_st16(ob + c, o);
-          }
-        }
-        uint64_t sum[2] = {0, 0};
-        const uint64_t scale = pair(w.scale2, w.scale2), minus = pair(-m2, -m2);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t p[16];
+          for (int j = 0; j < 32; j += 2) tm[(j / 2) & 3] = fmaxf(fmaxf(tm[(j / 2) & 3], __uint_as_float(v[c][j])), __uint_as_float(v[c][j + 1]));
+          return fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3]));
+        };
+        uint32_t p[16];
+        float sum;
+        auto probabilities = [&](int c) {  // p and their sum
+          uint64_t two[2] = {0, 0};
+          const uint64_t scale = pair(w.scale2, w.scale2), minus = pair(-m2, -m2);
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             uint64_t x = fma2(pair(__uint_as_float(v[c][2 * j]), __uint_as_float(v[c][2 * j + 1])), scale, minus);
@@ -372,37 +373,77 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
               const float2 f = unpair(x);
               x = pair(ex2(f.x), ex2(f.y));
             }
-            sum[j & 1] = add2(sum[j & 1], x);
+            two[j & 1] = add2(two[j & 1], x);
             const float2 f = unpair(x);
             p[j] = pack2<BF16>(f.x, f.y);
           }
-          // The products of the first 64 keys begin while the other probabilities are made.
-          if (c == 2) {
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&pf[2 * i]);
-          }
+          const float2 s0 = unpair(two[0]), s1 = unpair(two[1]);
+          sum = (s0.x + s0.y) + (s1.x + s1.y);
+        };
+        auto release = [&](int c) {  // the products of the first 32 keys begin while the others' probabilities are made
           tmem_st16(sb + c * 16, p);
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&pf[2 * i + c]);
+        };
+        // The first 32 probabilities are made against the maximum so far, beside the search for the tile's; where it has grown too much (a row's two
+        // threads have to agree, and the barrier tells both) they are made again.
+        tmem_ld32(sb, v[0]);
+        tmem_ld_wait();
+        tmem_ld32(sb + 32, v[1]);
+        hide(0);
+        float tmax = largest(0);
+        probabilities(0);
+        tmem_ld_wait();
+        hide(1);
+        tmax = fmaxf(tmax, largest(1));
+        if (agree(n == 0 || tmax * w.scale2 > m2 + PT_LAZY)) {
+          *mine = tmax;
+          meet_other();
+          const float nm = fmaxf(m2, fmaxf(tmax, *theirs) * w.scale2);
+          const bool grown = n == 0 || nm > m2 + PT_LAZY;
+          const float f = grown ? ex2(m2 - nm) : 1.f;
+          if (grown) m2 = nm;
+          l *= f;
+          if (n) {
+#pragma unroll 1
+            for (uint32_t c = 0; c < DH / 2; c += 16) {
+              tmem_ld16(ob + c, p);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) p[j] = __float_as_uint(__uint_as_float(p[j]) * f);
+              tmem_st16(ob + c, p);
+            }
+          }
+          tmem_ld32(sb, v[0]);
+          tmem_ld_wait();
+          hide(0);
+          probabilities(0);
         }
-        const float2 s0 = unpair(sum[0]), s1 = unpair(sum[1]);
-        l += (s0.x + s0.y) + (s1.x + s1.y);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&pf[2 * i + 1]);
+        l += sum;
+        release(0);
+        probabilities(1);
+        l += sum;
+        release(1);
       }
       if (ok && n) ok = __all_sync(0xffffffffu, poll(&fin[i], 0, abort_flag, 970 + i));
-      if (ok && k.tokens[i]) {
+      if (any_live) {
+        meet_other();  // the last maximum has been read
+        *mine = l;
+        meet_other();
+        l += *theirs;
+      }
+      if (ok && any_live) {
         tc_fence_after();
         const float inv = m2 == PT_LOWEST ? 0.f : 1.f / l;  // a row that has seen no score: zeros (its sum holds what 2^-126 is for minus infinity)
         uint16_t *out = static_cast<uint16_t *>(w.o) + (size_t)(k.s.first + token) * w.ld_o + (size_t)(k.g * group + row % group) * w.c.dim;
 #pragma unroll 1
-        for (uint32_t c = 0; c < DH; c += 32) {
+        for (uint32_t c = half * (DH / 2); c < (half + 1) * (DH / 2); c += 32) {
           uint32_t o[32];
           __syncwarp();
           if (n) {
-            tmem_ld32(ob + c, o);
+            tmem_ld32(lanes + 256 + i * 128 + c, o);
             tmem_ld_wait();
           }
           if (!live || c >= w.c.dim) continue;
@@ -412,7 +453,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             y[j] = n ? __uint_as_float(o[j]) : 0.f;
             z = fmaf(y[j], 0.f, z);
           }
-          if (z != 0.f)
+          if (z != 0.f && isfinite(l))
             paged_again<32>(w, BF16, false, k.b, k.s, k.g, (k.token0 + i * TT) * group + row, [&](int j) { return c + j; }, max(lim0, (int)(k.lo[i] * PT_KEYS)), lim1, m2, y);
 #pragma unroll
           for (int j = 0; j < 32; j += 8)
@@ -434,7 +475,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 
 template <int SD, bool BF16>
 int launch_tc(cudaStream_t stream, const PagedAttnArgs &w, uint32_t blocks) {
-  constexpr size_t smem = (size_t)(2 + PT_UNITS) * SD * PT_SLAB + 1024 + (2 * PT_UNITS + 11) * 8 + 16;
+  constexpr size_t smem = (size_t)(2 + PT_UNITS) * SD * PT_SLAB + (2 * PT_UNITS + 11) * 8 + 4 * PT_ROWS * 4 + 16;
   static bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
