@@ -532,13 +532,13 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const uint32_t r = m * 16 + gq + c * 8;
-          float y[DH / 16], z = 0.f;  // z: 0, or NaN
+          float z = 0.f;  // 0, or NaN
 #pragma unroll
-          for (int n = 0; n < (int)DH / 16; ++n) {
-            y[n] = o[m][n / 2][2 * c + (n & 1)];
-            z = fmaf(y[n], 0.f, z);
-          }
+          for (int n = 0; n < (int)DH / 16; ++n) z = fmaf(o[m][n / 2][2 * c + (n & 1)], 0.f, z);
           if (z != 0.f && r < rows && isfinite(l[m][c])) {
+            float y[DH / 16];
+#pragma unroll
+            for (int n = 0; n < (int)DH / 16; ++n) y[n] = o[m][n / 2][2 * c + (n & 1)];
             paged_again<DH / 16>(w, BF16, F32, g.b, g.s, g.g, g.R0 + r, [&](int n) { return warp * (DH / 4) + n / 2 * 8 + 2 * t4 + (n & 1); },
                                  max(lim0[m][c], (int)(g.t0 * PM_KEYS)), min(lim1[m][c], (int)(g.t1 * PM_KEYS)), mx[m][c], y);
 #pragma unroll

@@ -434,32 +434,51 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         meet_other();
         l += *theirs;
       }
-      if (ok && any_live) {
+      if (any_live) {
+        // Outputs go through shared memory (the tile's queries have been used): 16 bytes a lane straight from a row per lane are a line each, and took 5 us
+        // of a block, 6 more until they had drained and the next block could begin.
         tc_fence_after();
+        uint8_t *stage = qs + i * UNIT;
         const float inv = m2 == PT_LOWEST ? 0.f : 1.f / l;  // a row that has seen no score: zeros (its sum holds what 2^-126 is for minus infinity)
-        uint16_t *out = static_cast<uint16_t *>(w.o) + (size_t)(k.s.first + token) * w.ld_o + (size_t)(k.g * group + row % group) * w.c.dim;
+        if (ok && n) {
 #pragma unroll 1
-        for (uint32_t c = half * (DH / 2); c < (half + 1) * (DH / 2); c += 32) {
-          uint32_t o[32];
-          __syncwarp();
-          if (n) {
+          for (uint32_t c = half * (DH / 2); c < (half + 1) * (DH / 2); c += 32) {
+            uint32_t o[32];
+            __syncwarp();
             tmem_ld32(lanes + 256 + i * 128 + c, o);
             tmem_ld_wait();
-          }
-          if (!live || c >= w.c.dim) continue;
-          float y[32], z = 0.f;  // z: 0, or NaN
+            float y[32], z = 0.f;  // z: 0, or NaN
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            y[j] = n ? __uint_as_float(o[j]) : 0.f;
-            z = fmaf(y[j], 0.f, z);
-          }
-          if (z != 0.f && isfinite(l))
-            paged_again<32>(w, BF16, false, k.b, k.s, k.g, (k.token0 + i * TT) * group + row, [&](int j) { return c + j; }, max(lim0, (int)(k.lo[i] * PT_KEYS)), lim1, m2, y);
+            for (int j = 0; j < 32; ++j) {
+              y[j] = __uint_as_float(o[j]);
+              z = fmaf(y[j], 0.f, z);
+            }
+            if (z != 0.f && live && isfinite(l)) {
+              float x[32];  // in memory, which `y` stays out of
 #pragma unroll
-          for (int j = 0; j < 32; j += 8)
-            if (c + j < w.c.dim)
-              *reinterpret_cast<uint4 *>(out + c + j) = make_uint4(pack2<BF16>(y[j] * inv, y[j + 1] * inv), pack2<BF16>(y[j + 2] * inv, y[j + 3] * inv),
-                                                                   pack2<BF16>(y[j + 4] * inv, y[j + 5] * inv), pack2<BF16>(y[j + 6] * inv, y[j + 7] * inv));
+              for (int j = 0; j < 32; ++j) x[j] = y[j];
+              paged_again<32>(w, BF16, false, k.b, k.s, k.g, (k.token0 + i * TT) * group + row, [&](int j) { return c + j; }, max(lim0, (int)(k.lo[i] * PT_KEYS)), lim1, m2, x);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) y[j] = x[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 32; j += 8)
+              *reinterpret_cast<uint4 *>(stage + row * (DH * 2) + (((c + j) / 8 ^ (row & 7)) << 4)) =
+                  make_uint4(pack2<BF16>(y[j] * inv, y[j + 1] * inv), pack2<BF16>(y[j + 2] * inv, y[j + 3] * inv), pack2<BF16>(y[j + 4] * inv, y[j + 5] * inv),
+                             pack2<BF16>(y[j + 6] * inv, y[j + 7] * inv));
+          }
+        }
+        meet_other();
+        constexpr uint32_t LPR = DH / 8, RPP = 32 / LPR;  // lanes per row, rows per pass
+        const uint32_t e = lane % LPR, rows = k.tokens[i] * group;
+        if (ok && e * 8 < w.c.dim) {
+#pragma unroll 4
+          for (uint32_t x = 0; x < 16; x += RPP) {
+            const uint32_t r = quad * 32 + half * 16 + x + lane / LPR;
+            if (r >= rows) continue;
+            uint16_t *out = static_cast<uint16_t *>(w.o) + (size_t)(k.s.first + k.token0 + i * TT + r / group) * w.ld_o + (size_t)(k.g * group + r % group) * w.c.dim;
+            *reinterpret_cast<uint4 *>(out + e * 8) = n ? *reinterpret_cast<const uint4 *>(stage + r * (DH * 2) + ((e ^ (r & 7)) << 4)) : make_uint4(0, 0, 0, 0);
+          }
         }
       }
     }
