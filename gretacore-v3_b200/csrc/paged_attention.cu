@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
       if (!(g.first && g.last)) {
         const uint32_t c0 = (uint32_t)(g.begin / share), c1 = (uint32_t)((g.end - 1) / share);
         auto part = [&](uint32_t cta) {  // a CTA has at most one part that is no beginning of a list, and one that is
-          return w.parts + (size_t)(2 * cta + (cta == c0 ? 1 : 0)) * PAGED_PART;
+          return w.parts + (size_t)(2 * cta + (cta == c0 ? 1 : 0)) * PAGED_MMA_PART;
         };
         float *p = part(blockIdx.x);
 #pragma unroll
@@ -679,7 +679,7 @@ extern "C" {
 
 size_t greta_cuda_paged_attn_workspace_bytes(uint32_t dim) {
   (void)dim;
-  return PAGED_TICKETS + (size_t)2 * PAGED_MAX_CTAS * PAGED_PART * 4;
+  return PAGED_TICKETS + PAGED_PARTS * 4;
 }
 
 int greta_cuda_paged_attn(greta_stream_t stream, const greta_paged_cache *cache, const greta_ragged *rows, const void *q, int q_fmt, uint32_t ld_q, void *o,

@@ -18,22 +18,25 @@ struct PagedAttnArgs {
   uint32_t ld_q, ld_o, group, window;
   float scale2;      // scale * log2(e)
   uint32_t *tickets;  // [PAGED_MAX_CTAS], zero between calls
-  float *parts;       // PAGED_PART floats each
+  float *parts;       // PAGED_PARTS floats
   int *error;         // where a wait that gave up is reported
 };
 
-constexpr uint32_t PAGED_CTAS_PER_SM = 2, PAGED_MAX_CTAS = 512;
-constexpr uint32_t PAGED_TICKETS = 65536;  // bytes
-constexpr uint32_t PAGED_PART = 64 * (128 + 2);
+constexpr uint32_t PAGED_CTAS_PER_SM = 2, PAGED_MAX_CTAS = 512;  // of the form for few rows
+constexpr uint32_t PAGED_TC_CTAS = 192;                          // of the form for portions
+constexpr uint32_t PAGED_TICKETS = 65536;                        // bytes
+constexpr uint32_t PAGED_COUNTER = PAGED_TICKETS / 4 - 1;        // the word that blocks are drawn from
+constexpr uint32_t PAGED_MMA_PART = 64 * (128 + 2), PAGED_PART = 256 * (128 + 2);  // floats of a part of a row block
+constexpr size_t PAGED_PARTS = 2 * (size_t)(PAGED_MAX_CTAS * PAGED_MMA_PART > PAGED_TC_CTAS * PAGED_PART ? PAGED_MAX_CTAS * PAGED_MMA_PART : PAGED_TC_CTAS * PAGED_PART);
 
 int paged_attn_tc(cudaStream_t stream, PagedAttnArgs &w, uint32_t heads);  // paged_attention_tc.cu
 
 #ifdef __CUDACC__
 // Elements elem(0 .. N - 1) of row R's unnormalised output over the keys k0 .. k1 - 1 (all seen by the row), whose scores are taken against mx: again, where the
 // product with hidden keys' values left no finite numbers.  An element stays as it was if a value that the row sees is none either.  Rare and slow: a key at a time, by one
-// thread.  Not for rows whose sum of weights is no finite number: their outputs are none whatever the values are.
+// thread.  Inlined, and its arrays in local memory: around a call the caller's loops would keep their sums there.  Not for rows whose sum of weights is no finite number: their outputs are none whatever the values are.
 template <int N, typename Elem>
-__device__ __noinline__ void paged_again(const PagedAttnArgs &w, bool bf16, bool f32, uint32_t b, const PagedSeq &s, uint32_t g, uint32_t R, Elem elem, int k0, int k1, float mx,
+__device__ __forceinline__ void paged_again(const PagedAttnArgs &w, bool bf16, bool f32, uint32_t b, const PagedSeq &s, uint32_t g, uint32_t R, Elem elem, int k0, int k1, float mx,
                                          float (&y)[N]) {
   const uint32_t d = w.c.dim;
   const int32_t *table = w.c.table + (size_t)b * w.c.ld_table;
@@ -42,7 +45,7 @@ __device__ __noinline__ void paged_again(const PagedAttnArgs &w, bool bf16, bool
     return bf16 ? __uint_as_float((uint32_t)x << 16) : __half2float(__ushort_as_half(x));
   };
   uint32_t again = 0;
-#pragma unroll
+#pragma unroll 1
   for (int n = 0; n < N; ++n)
     if (elem(n) < d && !isfinite(y[n])) again |= 1u << n;
   auto row_of = [&](int j, size_t &row) {  // false: no page, values of zero
@@ -53,26 +56,26 @@ __device__ __noinline__ void paged_again(const PagedAttnArgs &w, bool bf16, bool
   size_t row;
   for (int j = k0; j < k1 && again; ++j) {
     if (!row_of(j, row)) continue;
-#pragma unroll
+#pragma unroll 1
     for (int n = 0; n < N; ++n)
       if (again >> n & 1 && !isfinite(value(w.c.v, row + elem(n)))) again &= ~(1u << n);
   }
   if (!again) return;
   const size_t qi = (size_t)(s.first + R / w.group) * w.ld_q + (size_t)(g * w.group + R % w.group) * d;
   float acc[N];
-#pragma unroll
+#pragma unroll 1
   for (int n = 0; n < N; ++n) acc[n] = 0.f;
   for (int j = k0; j < k1; ++j) {
     if (!row_of(j, row)) continue;
     float t = 0.f;
-#pragma unroll 8
+#pragma unroll 2
     for (uint32_t i = 0; i < d; ++i) t = fmaf(f32 ? static_cast<const float *>(w.q)[qi + i] : value(w.q, qi + i), value(w.c.k, row + i), t);
     const float p = exp2f(t * w.scale2 - mx);
-#pragma unroll
+#pragma unroll 1
     for (int n = 0; n < N; ++n)
       if (again >> n & 1) acc[n] = fmaf(p, value(w.c.v, row + elem(n)), acc[n]);
   }
-#pragma unroll
+#pragma unroll 1
   for (int n = 0; n < N; ++n)
     if (again >> n & 1) y[n] = acc[n];
 }

@@ -10,8 +10,10 @@
 // A row's sums are rescaled only when its maximum has grown by more than 2^8 (probabilities up to 2^8 fit every type); the scores' barrier of a key tile says that
 // the products of the one before are in, so the rows' own threads do that.
 #include <math.h>
+#include <stddef.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "mma_device.cuh"
 #include "paged_attention.cuh"
@@ -21,7 +23,11 @@ using namespace greta;
 
 namespace {
 
-constexpr uint32_t PT_ROWS = 128, PT_KEYS = 128, PT_THREADS = 576, PT_UNITS = 5, PT_TMEM = 512;
+constexpr uint32_t PT_ROWS = 128, PT_KEYS = 128, PT_THREADS = 576, PT_UNITS = 4, PT_TMEM = 512;
+constexpr uint32_t PT_LIST = 3;    // what a block costs besides its key tiles, in tiles: its queries, sums and outputs
+constexpr uint32_t PT_JOIN = 6;    // what joining the shares' parts costs, in tiles
+constexpr uint32_t PT_MAX_CTAS = PAGED_TC_CTAS;
+constexpr uint32_t PT_BARRIERS = 28, PT_SMALL = 3328;  // of a CTA; bytes of shared memory for them, exchanges, segments and words
 constexpr uint32_t PT_SLAB = 128 * 128;  // bytes of 64 elements of 128 rows
 constexpr int PT_EMULATED = 1;           // pairs of probabilities out of four that the FMA units make: the special-function unit's 16 a clock bound the tile otherwise
 constexpr float PT_LAZY = 8.f;           // log2 of what a row's maximum may grow by before its sums are rescaled
@@ -33,28 +39,49 @@ __device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *m
                : "memory");
 }
 // On the critical path: waits that the hardware ends (a time hint wakes late; testing without rest takes issue slots from the warps that compute).
-__device__ __noinline__ bool poll_slow(uint32_t bar, uint32_t parity, volatile int *abort_flag, int code) {
+// Shared memory is addressed with 32 bits: generic pointers take twice the registers, of which a row's scores leave none.
+__device__ __forceinline__ uint32_t lds(uint32_t at) {
+  uint32_t x;
+  asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(x) : "r"(at) : "memory");
+  return x;
+}
+__device__ __forceinline__ void sts(uint32_t at, uint32_t x) { asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(at), "r"(x) : "memory"); }
+__device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ bool test(uint32_t bar, uint32_t parity) {  // at once
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+// No call: what a caller's registers hold would go to local memory around it, and come back from the second-level cache when the wait is over.
+__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity, uint32_t abort_flag, int code) {
+  if (try_wait(bar, parity)) return true;
   const long long t0 = clock64();
-  for (;;) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if (*abort_flag) return false;
-    if (clock64() - t0 > WAIT_LIMIT_CYCLES) {
-      *abort_flag = code;
-      return false;
-    }
-  }
+  bool ok;
+  do {
+    ok = try_wait(bar, parity);
+    if (!ok && clock64() - t0 > WAIT_LIMIT_CYCLES) sts(abort_flag, code);
+  } while (!ok && !lds(abort_flag));
+  return ok;
 }
 __device__ __forceinline__ bool poll(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int code) {
-  if (mbar_try_wait(bar, parity)) return true;
-  return poll_slow(smem_u32(bar), parity, abort_flag, code);
+  return poll(smem_u32(bar), parity, smem_u32(const_cast<int *>(abort_flag)), code);
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
@@ -63,6 +90,17 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+__device__ __forceinline__ void tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+               : "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+               "r"(r[6]), "r"(r[7])
+               : "memory");
+}
 // Pairs of fp32 in one instruction.
 __device__ __forceinline__ uint64_t pair(float a, float b) {
   uint64_t r;
@@ -98,389 +136,793 @@ __device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
   return pair(__int_as_float(__float_as_int(y.x) + (__float_as_int(e.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(e.y) << 23)));
 }
 
-// A block of rows of one sequence and KV head, and the key tiles of its two halves.
+// A block of rows of one sequence and KV head: its tokens as two halves, and the key tiles lo .. hi - 1 that each sees; t0 .. t1 - 1 is both.
 struct Block {
-  uint32_t b, g, token0, t0, t1;      // tiles t0 .. t1 - 1 of either half
-  uint32_t tokens[2], lo[2], hi[2];   // of half i: its tokens, tiles lo .. hi - 1
+  uint32_t token0, tokens[2], lo[2], hi[2], t0, t1;
+};
+__device__ __forceinline__ Block block_of(const PagedSeq &s, uint32_t j, uint32_t TT, uint32_t window) {
+  Block k;
+  k.token0 = j * 2 * TT;
+#pragma unroll
+  for (uint32_t i = 0; i < 2; ++i) {
+    const uint32_t first = k.token0 + i * TT;
+    k.tokens[i] = first < s.rows ? min(TT, s.rows - first) : 0;
+    const int pos = s.pos0 + (int)first, end = pos + (int)k.tokens[i];  // positions pos .. end - 1
+    const int from = window ? pos - (int)window + 1 : 0;
+    k.lo[i] = k.tokens[i] == 0 ? k.lo[0] : from > 0 ? (uint32_t)from / PT_KEYS : 0;
+    k.hi[i] = k.tokens[i] && end > 0 ? ((uint32_t)end + PT_KEYS - 1) / PT_KEYS : k.lo[i];
+  }
+  // The second half's tiles begin and end no earlier than the first's, and there is none between them: its first row follows the first half's last.
+  k.t0 = k.lo[0];
+  k.t1 = max(k.hi[0], k.hi[1]);
+  return k;
+}
+// What a block costs: its tiles (one where it sees no key) and PT_LIST for its beginning and end.
+__device__ __forceinline__ uint32_t places_of(const Block &k) { return max(1u, k.t1 - k.t0) + PT_LIST; }
+
+// What a CTA works on at a time: a block of a KV head, its tiles clipped to k.t0 .. k.t1 - 1.
+struct Segment {
+  Block k;
   PagedSeq s;
+  uint32_t b, g;
+  uint32_t whole, ragged;  // all of the block; the last tile is the last of the sequence and holds rows behind its end
+  uint32_t c0, c1;         // the CTAs that share the block
+  uint32_t clear0[2], clear1[2];  // of a half: the tiles that all its rows see whole
+  int pos[2];              // of a half: its first row's position
+  uint32_t more;           // 0: there was none
+};
+
+// What is to be done, in the order of its places: sequences, their blocks from the last (and longest) to the first, KV heads.  Used by all lanes of a warp.
+struct Finder {
+  const PagedAttnArgs &w;
+  const uint64_t *prefix;  // places (or blocks) in front of a sequence, and of the end
+  const PagedSeq *seqs;
+  const uint64_t share;    // places of each CTA
+  const uint32_t TT, G, lane;
+  uint64_t at, stop, begin = 0;  // the next place, the end of the CTA's; the first place of the block that `at` lies in
+  uint32_t cur = 0, jj = 0, kvh = 0;  // that block: sequence, number from the last, KV head
+  bool found = false;
+
+  __device__ Finder(const PagedAttnArgs &w, const uint64_t *prefix, const PagedSeq *seqs, uint64_t share)
+      : w(w), prefix(prefix), seqs(seqs), share(share), TT(PT_ROWS / w.group), G(w.c.kv_heads), lane(threadIdx.x & 31) {
+    at = min(prefix[w.r.batch], share * blockIdx.x);
+    stop = min(prefix[w.r.batch], at + share);
+  }
+  __device__ uint32_t blocks_of(const PagedSeq &s) const { return (s.rows + 2 * TT - 1) / (2 * TT); }
+  __device__ uint32_t seq_at(uint64_t x) const {  // prefix[b] <= x < prefix[b + 1]
+    uint32_t lo = 0, hi = w.r.batch;
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (prefix[mid] <= x)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    return lo;
+  }
+  __device__ void finish(Segment &g) const {
+    g.whole = g.c0 == g.c1;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int first = g.s.pos0 + (int)(g.k.token0 + i * TT), last = first + (int)g.k.tokens[i] - 1;
+      g.pos[i] = first;
+      g.clear0[i] = w.window && last >= (int)w.window ? (uint32_t)(last - (int)w.window + PT_KEYS) / PT_KEYS : 0;
+      g.clear1[i] = first < 0 ? 0 : (uint32_t)(first + 1) / PT_KEYS;
+    }
+  }
+  __device__ bool ragged(const Segment &g) const { return g.k.t1 > g.k.t0 && (int)(g.k.t1 * PT_KEYS) > g.s.pos0 + (int)g.s.rows; }
+  // A whole block by its number.
+  __device__ void block(uint32_t x, Segment &g) const {
+    g.b = seq_at(x);
+    g.s = seqs[g.b];
+    const uint32_t in = x - (uint32_t)prefix[g.b];
+    g.g = in % G;
+    g.k = block_of(g.s, blocks_of(g.s) - 1 - in / G, TT, w.window);
+    g.c0 = g.c1 = 0;
+    g.ragged = ragged(g);
+    finish(g);
+  }
+  __device__ void search() {  // the share's beginning: which sequence, and which of its blocks, 32 at a time
+    cur = seq_at(at);
+    const PagedSeq s = seqs[cur];
+    const uint32_t blocks = blocks_of(s);
+    uint64_t before = prefix[cur];
+    for (uint32_t j0 = 0; !found; j0 += 32) {
+      const uint32_t mine = j0 + lane < blocks ? places_of(block_of(s, blocks - 1 - j0 - lane, TT, w.window)) * G : 0;
+      uint32_t v = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
+      }
+      const uint32_t hit = __ballot_sync(0xffffffffu, before + v > at);
+      found = hit || j0 + 32 >= blocks;
+      if (found) {
+        const int l = hit ? __ffs(hit) - 1 : 0;
+        jj = j0 + l;
+        const uint32_t first = __shfl_sync(0xffffffffu, v - mine, l), each = __shfl_sync(0xffffffffu, mine, l) / G;
+        kvh = (uint32_t)((at - before - first) / each);
+        begin = before + first + (uint64_t)kvh * each;
+      }
+      before += __shfl_sync(0xffffffffu, v, 31);
+    }
+  }
+  // The next part of the CTA's share.
+  __device__ bool part(Segment &g) {
+    while (at < stop) {
+      if (!found) search();
+      g.b = cur;
+      g.g = kvh;
+      g.s = seqs[cur];
+      const uint32_t blocks = blocks_of(g.s);
+      g.k = block_of(g.s, blocks - 1 - jj, TT, w.window);
+      const uint32_t tiles = g.k.t1 - g.k.t0, places = places_of(g.k), p = (uint32_t)(at - begin), n = (uint32_t)min((uint64_t)(places - p), stop - at);
+      const uint64_t first = begin + PT_LIST, end = begin + places;
+      at += n;
+      if (at == end) {  // on to the next block
+        begin = end;
+        if (++kvh == G) {
+          kvh = 0;
+          if (++jj == blocks) {
+            jj = 0;
+            while (++cur < w.r.batch && prefix[cur + 1] == prefix[cur]) {
+            }
+          }
+        }
+      }
+      const uint32_t a = max(p, PT_LIST) - PT_LIST, z = max(p + n, PT_LIST) - PT_LIST;
+      if (a == z) continue;
+      g.c0 = (uint32_t)(first / share);
+      g.c1 = (uint32_t)((end - 1) / share);
+      const uint32_t t0 = g.k.t0 + min(a, tiles), t1 = g.k.t0 + min(z, tiles);
+      const bool to_end = t1 == g.k.t1;
+      g.k.t0 = t0;
+      g.k.t1 = t1;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        g.k.lo[i] = min(max(g.k.lo[i], t0), t1);
+        g.k.hi[i] = max(min(g.k.hi[i], t1), g.k.lo[i]);
+      }
+      g.ragged = to_end && ragged(g);
+      finish(g);
+      return true;
+    }
+    return false;
+  }
 };
 
 template <int SD, bool BF16>
 __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_constant__ PagedAttnArgs w) {
   constexpr uint32_t DH = SD * 64, UNIT = SD * PT_SLAB;
-  extern __shared__ __align__(1024) uint8_t paged_tc_smem[];  // alignment of the swizzled tiles; there is no room to align it by hand
-  uint8_t *smem = paged_tc_smem;
-  uint8_t *qs = smem, *ring = qs + 2 * UNIT;  // queries of both tiles; keys and values in turn
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint8_t *qs = smem, *ring = qs + 2 * UNIT;  // queries of both halves, then their outputs; keys and values in turn
   uint64_t *bars = reinterpret_cast<uint64_t *>(ring + PT_UNITS * UNIT);
-  uint64_t *full = bars, *empty = full + PT_UNITS, *qf = empty + PT_UNITS, *sf = qf + 1, *pf = sf + 2, *vl = pf + 4, *vz = vl + 1, *fin = vz + 1;  // vl: the last values have come; vz: and hold zeros behind the sequence
-  float *meet = reinterpret_cast<float *>(fin + 2);  // [tile][half][row]: what the two threads of a row tell each other
-  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(meet + 4 * PT_ROWS), *place = tmem_slot + 1;  // place: sequence, block
-  volatile int *abort_flag = reinterpret_cast<volatile int *>(place + 2);
+  constexpr uint32_t FULL = 0, EMPTY = FULL + PT_UNITS, QF = EMPTY + PT_UNITS, QE = QF + 2, SF = QE + 2, PF = SF + 2, FIN = PF + 4, VL = FIN + 2, VZ = VL + 1, NF = VZ + 2, NE = NF + 2;
+  static_assert(NE + 2 <= PT_BARRIERS, "barriers");
+  uint64_t *full = bars + FULL, *empty = bars + EMPTY, *qf = bars + QF, *qe = bars + QE, *sf = bars + SF, *pf = bars + PF, *fin = bars + FIN;
+  uint64_t *vl = bars + VL, *vz = bars + VZ;  // the last values of a ragged sequence have come; and hold zeros behind its end (two in turn: one may follow the other at once)
+  uint64_t *nf = bars + NF, *ne = bars + NE;  // the next segment is there; is done with
+  // Behind the barriers: [half][column half][row] floats that the two threads of a row tell each other; [row] its token and head (divisions by the group,
+  // once); two segments (warp 0 finds them, one ahead; the others leave in them what they need late); words; and what depends on the batch.
+  constexpr uint32_t MEET = PT_BARRIERS * 8, ROWS = MEET + 4 * PT_ROWS * 4, SEGMENTS = ROWS + PT_ROWS * 4, WORDS = SEGMENTS + 2 * sizeof(Segment);
+  uint8_t *small = reinterpret_cast<uint8_t *>(bars);
+  Segment *segments = reinterpret_cast<Segment *>(small + SEGMENTS);
+  uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(small + WORDS), *ticket = tmem_slot + 1, *limits = ticket + 1;  // limits: cost of the largest and of the smallest block
+  volatile int *abort_flag = reinterpret_cast<volatile int *>(limits + 2);
+  constexpr uint32_t ABORT = WORDS + 16;
+  uint64_t *prefix = reinterpret_cast<uint64_t *>(small + PT_SMALL);  // [batch + 1]: places (or blocks) in front of a sequence
+  PagedSeq *seqs = reinterpret_cast<PagedSeq *>(prefix + w.r.batch + 1);
+  static_assert(WORDS + 32 <= PT_SMALL, "small things");
+  const uint32_t sm = smem_u32(bars);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-  const uint32_t group = w.group, TT = PT_ROWS / group;
+  const uint32_t group = w.group, TT = PT_ROWS / group, G = w.c.kv_heads, N = gridDim.x;
 
   if (threadIdx.x == 0) {
     for (uint32_t i = 0; i < PT_UNITS; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
-    mbar_init(qf, 1);
-    mbar_init(vl, 1);
-    mbar_init(vz, 1);
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&qf[i], 1);
+      mbar_init(&qe[i], 9);  // the half's warps, and the one that issues
       mbar_init(&sf[i], 1);
       mbar_init(&pf[2 * i], 8);  // the first and the second 32 keys of both warps of a row
       mbar_init(&pf[2 * i + 1], 8);
       mbar_init(&fin[i], 1);
+      mbar_init(&nf[i], 1);
+      mbar_init(&ne[i], 17);
     }
-    place[0] = 0xffffffffu;
-    *abort_flag = smem_u32(smem) % 1024 ? 999 : 0;
+    mbar_init(vl, 1);
+    mbar_init(vz, 1);
+    mbar_init(vz + 1, 1);
+    limits[0] = 0;
+    limits[1] = 0xffffffffu;
+    *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&w.k) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&w.v) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&w.qm) : "memory");
   }
+  if (threadIdx.x >= 64 && threadIdx.x < 64 + PT_ROWS) {
+    const uint32_t row = threadIdx.x - 64;
+    sts(sm + ROWS + row * 4, row / group | row % group << 16);
+  }
   if (warp == 1) {
     tmem_alloc(tmem_slot, PT_TMEM);
     tmem_relinquish();
   }
+  pdl_launch_dependents();
+  pdl_wait();
+  // ---- what there is to do: every sequence's rows, the places of its blocks, their largest and smallest
+  const uint32_t max_len = w.c.ld_table * w.c.page;
+  for (uint32_t b = threadIdx.x; b < w.r.batch; b += PT_THREADS) seqs[b] = paged_seq(w.r, max_len, b);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  pdl_launch_dependents();
-  pdl_wait();
-
-  // ---- which block: sequences in order, the last rows of each (the longest) first, KV heads side by side
-  const uint32_t max_len = w.c.ld_table * w.c.page, heads_kv = w.c.kv_heads;
-  if (warp == 0 && *abort_flag == 0) {
-    uint32_t before = 0;
-    const uint32_t mine = blockIdx.x / heads_kv;
-    for (uint32_t b0 = 0; b0 < w.r.batch; b0 += 32) {
-      uint32_t n = 0;
-      if (b0 + lane < w.r.batch) n = (paged_seq(w.r, max_len, b0 + lane).rows + 2 * TT - 1) / (2 * TT);
-      uint32_t v = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += x;
-      }
-      if (mine >= before + v - n && mine < before + v) {
-        place[0] = b0 + lane;
-        place[1] = before + v - 1 - mine;
-      }
-      before += __shfl_sync(0xffffffffu, v, 31);
+  for (uint32_t b = warp; b < w.r.batch; b += PT_THREADS / 32) {
+    const PagedSeq s = seqs[b];
+    const uint32_t blocks = (s.rows + 2 * TT - 1) / (2 * TT);
+    uint32_t sum = 0, most = 0, least = 0xffffffffu;  // places of 2^24 rows' blocks over 2^24 tiles each would not fit, in 32 bits; nor would the work end
+    for (uint32_t j = lane; j < blocks; j += 32) {
+      const uint32_t n = places_of(block_of(s, j, TT, w.window));
+      sum += n;
+      most = max(most, n);
+      least = min(least, n);
+    }
+    const uint32_t all = __reduce_add_sync(0xffffffffu, sum);
+    most = __reduce_max_sync(0xffffffffu, most);
+    least = __reduce_min_sync(0xffffffffu, least);
+    if (lane == 0) {
+      prefix[b + 1] = (uint64_t)all * G | (uint64_t)blocks << 48;
+      atomicMax(&limits[0], most);
+      atomicMin(&limits[1], least);
     }
   }
   __syncthreads();
-  Block k;
-  k.b = place[0];
-  if (k.b != 0xffffffffu) {
-    k.g = blockIdx.x % heads_kv;
-    k.s = paged_seq(w.r, max_len, k.b);
-    k.token0 = place[1] * 2 * TT;
-#pragma unroll
-    for (uint32_t i = 0; i < 2; ++i) {
-      const uint32_t first = k.token0 + i * TT;
-      k.tokens[i] = first < k.s.rows ? min(TT, k.s.rows - first) : 0;
-      const int pos = k.s.pos0 + (int)first, end = pos + (int)k.tokens[i];  // positions pos .. end - 1
-      const int from = w.window ? pos - (int)w.window + 1 : 0;
-      k.lo[i] = k.tokens[i] == 0 ? k.lo[0] : from > 0 ? (uint32_t)from / PT_KEYS : 0;
-      k.hi[i] = k.tokens[i] && end > 0 ? ((uint32_t)end + PT_KEYS - 1) / PT_KEYS : k.lo[i];
+  if (warp == 0) {
+    uint64_t places = 0;
+    uint32_t blocks = 0;
+    for (uint32_t b = lane; b < w.r.batch; b += 32) {
+      places += prefix[b + 1] & 0xffffffffffffull;
+      blocks += (uint32_t)(prefix[b + 1] >> 48);
     }
-    // The second half's tiles begin and end no earlier than the first's, and there is none between them: its first row follows the first half's last.
-    k.t0 = k.lo[0];
-    k.t1 = max(k.hi[0], k.hi[1]);
-    const int last = k.s.pos0 + (int)k.s.rows;  // behind the sequence's last position
-    const bool ragged = k.t1 > k.t0 && (int)(k.t1 * PT_KEYS) > last;  // its last tile holds rows behind it
-
-    const bool leader = elect_one();
-    if (warp == 0) {
-      const uint32_t box = min(w.c.page, PT_KEYS), boxes = PT_KEYS / box;
-      const int32_t *table = w.c.table + (size_t)k.b * w.c.ld_table;
-      uint32_t it = 0;
-      bool ok = true;
-      if (leader) {
-        mbar_arrive_expect_tx(qf, (k.tokens[1] ? 2 : 1) * SD * 128 * group * TT);
-        for (uint32_t i = 0; i < 2; ++i)
-          for (uint32_t c = 0; c < SD && k.tokens[i]; ++c)
-            tma_load_3d(qs + i * UNIT + c * PT_SLAB, &w.qm, (int)(c * 64), (int)(k.g * group), (int)(k.s.first + k.token0 + i * TT), qf);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      places += __shfl_xor_sync(0xffffffffu, places, o);
+      blocks += __shfl_xor_sync(0xffffffffu, blocks, o);
+    }
+    // Whole blocks, taken one by one, end when the last one taken does; equal shares of all places end together, but their blocks have to be joined.
+    const uint64_t ends = (uint64_t)blocks * G <= N ? limits[0] : max((uint64_t)limits[0], places / N + limits[1]);
+    const bool shares = ends > places / N + PT_JOIN;
+    uint64_t sum = 0;
+    for (uint32_t b0 = 0; b0 < w.r.batch; b0 += 32) {
+      uint64_t v = 0;
+      if (b0 + lane < w.r.batch) v = shares ? prefix[b0 + lane + 1] & 0xffffffffffffull : (prefix[b0 + lane + 1] >> 48) * G;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint64_t x = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += x;
       }
-      auto page_of = [&](uint32_t t) {
-        const uint32_t p = t * PT_KEYS + lane * box;
-        return lane < boxes && t < k.t1 && p < k.s.len ? __ldcg(table + p / w.c.page) : -1;
-      };
-      int next = page_of(k.t0);
-      for (uint32_t t = k.t0; t < k.t1; ++t) {
-        const int id = next;
-        next = page_of(t + 1);
+      if (b0 + lane < w.r.batch) prefix[b0 + lane + 1] = sum + v;
+      sum += __shfl_sync(0xffffffffu, v, 31);
+    }
+    if (lane == 0) {
+      prefix[0] = 0;
+      limits[0] = shares;
+    }
+  }
+  __syncthreads();
+  const bool shares = limits[0] != 0;
+  const uint64_t total = prefix[w.r.batch], share = shares ? max((total + N - 1) / N, (uint64_t)PT_LIST + 2) : 0;
+  // The next segment, in shared memory until `done`.  Warps that meet in barriers go on or end together (`together`), whatever became of a wait.
+  uint32_t had = 0;
+  auto next = [&](bool &ok, auto together) -> uint32_t {  // its address, 0: there is none
+    const uint32_t x = had & 1, at = sm + SEGMENTS + x * (uint32_t)sizeof(Segment);
+    if (ok) ok = __all_sync(0xffffffffu, poll(sm + (NF + x) * 8, had >> 1 & 1, sm + ABORT, 980 + x));
+    ok = together(ok);
+    return ok && lds(at + offsetof(Segment, more)) ? at : 0;
+  };
+  auto done = [&] {
+    __syncwarp();
+    if (lane == 0) arrive(sm + (NE + (had & 1)) * 8);
+    ++had;
+  };
+
+  const bool leader = elect_one();
+  if (warp == 0) {
+    Finder find(w, prefix, seqs, share);
+    const uint32_t box = min(w.c.page, PT_KEYS), boxes = PT_KEYS / box;
+    uint32_t it = 0, loads0 = 0, loads1 = 0, tails = 0, handed = 0;
+    bool ok = true;
+    // Blocks are taken from a counter in the workspace as the copies of the one before end; the CTA that draws the last number sets it back.
+    auto take = [&]() -> const Segment * {
+      const uint32_t x = handed & 1;
+      Segment g;
+      bool more;
+      if (shares) {
+        more = find.part(g);
+      } else {
+        uint32_t id = blockIdx.x;
+        if (handed) {
+          if (lane == 0) {
+            id = atomicAdd(w.tickets + PAGED_COUNTER, 1u);
+            if (id + 1 == total) w.tickets[PAGED_COUNTER] = 0;
+            id += N;
+          }
+          id = __shfl_sync(0xffffffffu, id, 0);
+        }
+        more = id < total;
+        if (more) find.block(id, g);
+      }
+      if (ok) ok = poll(&ne[x], (handed >> 1 & 1) ^ 1, abort_flag, 985);
+      ++handed;
+      __syncwarp();
+      if (lane == 0) {
+        segments[x] = g;
+        segments[x].more = more;
+        mbar_arrive(&nf[x]);
+      }
+      __syncwarp();
+      return more ? segments + x : nullptr;
+    };
+    auto page_of = [&](const Segment *g, uint32_t t, uint32_t end) {
+      const uint32_t p = t * PT_KEYS + lane * box;
+      return lane < boxes && t < end && p < g->s.len ? __ldcg(w.c.table + (size_t)g->b * w.c.ld_table + p / w.c.page) : -1;
+    };
+    // Queries of the two halves take the place of the block before's outputs, each when those have left; the copies of keys and values do not wait for that.
+    const Segment *asking = nullptr;
+    uint32_t asked = 0;  // bits: halves whose queries have been asked for
+    auto ask = [&](uint32_t i, uint32_t &loads) {
+      if (asking->k.tokens[i] == 0) {
+        asked |= 1u << i;
+      } else if (!(asked >> i & 1) && __any_sync(0xffffffffu, test(sm + (QE + i) * 8, (loads & 1) ^ 1))) {
+        asked |= 1u << i;
+        ++loads;
+        if (leader && ok) {
+          mbar_arrive_expect_tx(&qf[i], SD * 128 * group * TT);
+          for (uint32_t c = 0; c < SD; ++c)
+            tma_load_3d(qs + i * UNIT + c * PT_SLAB, &w.qm, (int)(c * 64), (int)(asking->g * group), (int)(asking->s.first + asking->k.token0 + i * TT), &qf[i]);
+        }
+        __syncwarp();
+      }
+    };
+    auto ask_both = [&] {
+      if (asked != 3) {
+        ask(0, loads0);
+        ask(1, loads1);
+      }
+    };
+    // Until the barrier's phase is over (bar 0: until both halves' queries have been asked for).
+    auto wait_asking = [&](uint32_t bar, uint32_t parity, int code) {
+      const long long since = clock64();
+      bool over = false;
+      while (ok && !over) {
+        ask_both();
+        over = bar ? __all_sync(0xffffffffu, asked == 3 ? try_wait(bar, parity) : test(bar, parity)) : asked == 3;
+        if (!over && clock64() - since > WAIT_LIMIT_CYCLES) sts(sm + ABORT, code);
+        __syncwarp();
+        if (!over && lds(sm + ABORT)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+      }
+    };
+    uint32_t tail_at = 0, tail_from = PT_KEYS;  // the unit with a ragged sequence's last values, and where its zeros begin
+    auto zeros = [&] {
+      if (tail_from < PT_KEYS) {
+        if (ok) ok = mbar_wait(vl, tails & 1, abort_flag, 950);
+        __syncwarp();
+        ++tails;
+        if (ok) {
+          const uint32_t n = (PT_KEYS - tail_from) * 8;
+          for (uint32_t i = lane; i < n * SD; i += 32) {
+            *reinterpret_cast<uint4 *>(ring + tail_at * UNIT + i / n * PT_SLAB + tail_from * 128 + i % n * 16) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (leader && ok) mbar_arrive(vz + (tails & 1 ^ 1));
+        tail_from = PT_KEYS;
+      }
+    };
+    const Segment *g = take();
+    bool first = true;
+    while (g) {
+      const uint32_t t0 = g->k.t0, t1 = g->k.t1;
+      int ahead = page_of(g, t0, t1);
+      asking = g;
+      asked = 0;
+      if (first) ask_both();
+      for (uint32_t t = t0; t < t1; ++t) {
+        const int id = ahead;
+        ahead = page_of(g, t + 1, t1);
         const uint32_t p = t * PT_KEYS + lane * box;
         // no page: rows in front of the pool, which read as zeros
-        const int row = (uint32_t)id < w.c.pages ? (int)(((uint32_t)id * heads_kv + k.g) * w.c.page + p % w.c.page) : -(int)PT_KEYS;
+        const int row = (uint32_t)id < w.c.pages ? (int)(((uint32_t)id * G + g->g) * w.c.page + p % w.c.page) : -(int)PT_KEYS;
+        const bool last = t + 1 == t1 && g->ragged;
 #pragma unroll
         for (uint32_t kv = 0; kv < 2; ++kv, ++it) {
           const uint32_t st = it % PT_UNITS;
-          if (ok) ok = poll(&empty[st], ((it / PT_UNITS) & 1) ^ 1, abort_flag, 900 + st);
+          wait_asking(sm + (EMPTY + st) * 8, ((it / PT_UNITS) & 1) ^ 1, 900 + st);
           __syncwarp();
-          uint64_t *bar = kv && ragged && t + 1 == k.t1 ? vl : &full[st];
+          uint64_t *bar = kv && last ? vl : &full[st];
           if (leader && ok) mbar_arrive_expect_tx(bar, UNIT);
+          if (leader && ok && kv && last) mbar_arrive(&full[st]);  // its phase goes on without it
           __syncwarp();
           if (ok && lane < boxes)
             for (uint32_t c = 0; c < SD; ++c) tma_load_2d(ring + st * UNIT + c * PT_SLAB + lane * box * 128, kv ? &w.v : &w.k, (int)(c * 64), row, bar);
         }
-      }
-      if (ragged) {  // what the last page holds behind the sequence's end: zeros
-        if (ok) ok = mbar_wait(vl, 0, abort_flag, 950);
-        __syncwarp();
-        const uint32_t from = (uint32_t)max(0, last - (int)((k.t1 - 1) * PT_KEYS));
-        if (ok) {
-          for (uint32_t i = lane; i < (PT_KEYS - from) * 8 * SD; i += 32)
-            *reinterpret_cast<uint4 *>(ring + (it - 1) % PT_UNITS * UNIT + i / ((PT_KEYS - from) * 8) * PT_SLAB + from * 128 + i % ((PT_KEYS - from) * 8) * 16) =
-                make_uint4(0, 0, 0, 0);
+        if (t == t0) zeros();  // of the block before, behind the first copies of this one
+        if (last) {
+          tail_at = (it - 1) % PT_UNITS;
+          tail_from = (uint32_t)max(0, g->s.pos0 + (int)g->s.rows - (int)(t * PT_KEYS));
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (leader && ok) mbar_arrive(vz);
       }
-      if (leader && *abort_flag) drain_copies(full, it, PT_UNITS);
-      if (leader && *abort_flag) drain_copies(qf, 1, 1);
-      if (leader && *abort_flag) drain_copies(vl, ragged ? 1 : 0, 1);
-    } else if (warp == 1) {
-      constexpr uint32_t idesc_s = BF16 ? instr_desc_bf16(PT_ROWS, PT_KEYS) : instr_desc_f16(PT_ROWS, PT_KEYS);
-      constexpr uint32_t idesc_o = (BF16 ? instr_desc_bf16(PT_ROWS, DH) : instr_desc_f16(PT_ROWS, DH)) | (1u << 16);  // values: keys are the rows of memory (N-major operand)
-      const uint32_t q_lo = smem_desc_lo(smem_u32(qs)), k_lo = smem_desc_lo(smem_u32(ring));
-      const uint32_t v_lo = ((smem_u32(ring) >> 4) & 0x3FFFu) | ((PT_SLAB >> 4) << 16);  // 64-element groups are a slab apart
-      bool ok = true;
-      if (ok) ok = mbar_wait(qf, 0, abort_flag, 910);
-      __syncwarp();
-      auto scores = [&](uint32_t i, uint32_t t) {  // of half i with key tile t
-        if (leader && ok) {
-          tc_fence_after();
-          const uint32_t st = 2 * (t - k.t0) % PT_UNITS;
-#pragma unroll
-          for (uint32_t k16 = 0; k16 < DH / 16; ++k16)
-            umma_f16(tmem + i * 128, q_lo + (i * UNIT + (k16 / 4) * PT_SLAB) / 16 + (k16 & 3) * 2, k_lo + (st * UNIT + (k16 / 4) * PT_SLAB) / 16 + (k16 & 3) * 2,
-                     SMEM_DESC_HI_SW128, idesc_s, k16 ? 1u : 0u);
-          umma_commit(&sf[i]);
-        }
-      };
-      uint32_t np[2] = {0, 0};  // key tiles whose products with the values are under way
-      for (uint32_t t = k.t0; t <= k.t1; ++t) {
+      if (t0 == t1) zeros();
+      wait_asking(0, 0, 990);
+      first = false;
+      g = take();
+    }
+    zeros();
+    if (leader && *abort_flag) drain_copies(full, it, PT_UNITS);
+    if (leader && *abort_flag) drain_copies(qf, loads0, 1);
+    if (leader && *abort_flag) drain_copies(qf + 1, loads1, 1);
+    if (leader && *abort_flag) drain_copies(vl, tails, 1);
+  } else if (warp == 1) {
+    constexpr uint32_t idesc_s = BF16 ? instr_desc_bf16(PT_ROWS, PT_KEYS) : instr_desc_f16(PT_ROWS, PT_KEYS);
+    constexpr uint32_t idesc_o = (BF16 ? instr_desc_bf16(PT_ROWS, DH) : instr_desc_f16(PT_ROWS, DH)) | (1u << 16);  // values: keys are the rows of memory (N-major operand)
+    const uint32_t q_lo = smem_desc_lo(smem_u32(qs)), k_lo = smem_desc_lo(smem_u32(ring));
+    const uint32_t v_lo = ((smem_u32(ring) >> 4) & 0x3FFFu) | ((PT_SLAB >> 4) << 16);  // 64-element groups are a slab apart
+    bool ok = true;
+    uint32_t base = 0, tails = 0;  // units before this segment; ragged ends so far
+    // A half: its tiles in this segment, products with the values made in it, phases of its barriers.  Two of them by name and the code for each: an array that is
+    // indexed lies in local memory, whose loads stood between the products.
+    struct Half {
+      uint32_t lo, hi, made, tiles, loads;
+    } first{}, second{};
+    while (next(ok, [](bool x) { return x; })) {
+      const uint32_t at = sm + SEGMENTS + (had & 1) * (uint32_t)sizeof(Segment);
+      const uint32_t t0 = lds(at + offsetof(Segment, k.t0)), t1 = lds(at + offsetof(Segment, k.t1));
+      const bool ragged = lds(at + offsetof(Segment, ragged));
+      first.lo = lds(at + offsetof(Segment, k.lo)), first.hi = lds(at + offsetof(Segment, k.hi)), first.made = 0;
+      second.lo = lds(at + offsetof(Segment, k.lo) + 4), second.hi = lds(at + offsetof(Segment, k.hi) + 4), second.made = 0;
+      for (uint32_t t = t0; t <= t1; ++t) {
         // outputs of tile t - 1, scores of tile t, half by half
-        const uint32_t ik = 2 * (t - k.t0), iv = 2 * (t - 1 - k.t0) + 1;
-        const bool kt = t < k.t1, vt = t > k.t0;
+        const uint32_t ik = base + 2 * (t - t0), iv = ik - 1, sk = ik % PT_UNITS, sv = iv % PT_UNITS;
+        const bool kt = t < t1, vt = t > t0;
         bool have_k = false, have_v = false;
-#pragma unroll
-        for (uint32_t i = 0; i < 2; ++i) {
-          if (vt && t - 1 >= k.lo[i] && t - 1 < k.hi[i]) {
+        auto products = [&](auto I, Half &h) {
+          constexpr uint32_t i = I.value;
+          if (vt && t - 1 >= h.lo && t - 1 < h.hi) {
             if (!have_v) {
-              if (ok) ok = ragged && t == k.t1 ? poll(vz, 0, abort_flag, 921) : poll(&full[iv % PT_UNITS], (iv / PT_UNITS) & 1, abort_flag, 920);
+              if (ok) ok = ragged && t == t1 ? poll(sm + (VZ + (tails & 1)) * 8, tails >> 1 & 1, sm + ABORT, 921) : poll(sm + (FULL + sv) * 8, (iv / PT_UNITS) & 1, sm + ABORT, 920);
               have_v = true;
             }
 #pragma unroll
             for (uint32_t part = 0; part < 2; ++part) {
-              if (ok) ok = poll(&pf[2 * i + part], np[i] & 1, abort_flag, 930 + 2 * i + part);
+              if (ok) ok = poll(sm + (PF + 2 * i + part) * 8, h.tiles & 1, sm + ABORT, 930 + 2 * i + part);
               __syncwarp();
               if (leader && ok) {
                 tc_fence_after();
 #pragma unroll
                 for (uint32_t x = 0; x < 4; ++x) {
-                  const uint32_t k16 = (x >> 1) * 4 + part * 2 + (x & 1);  // a half's probabilities lie in the first 32 of its own 64 columns of scores
-                  umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + (x >> 1) * 64 + (part * 2 + (x & 1)) * 8, v_lo + (iv % PT_UNITS) * (UNIT / 16) + k16 * (2048 >> 4),
-                              SMEM_DESC_HI_SW128, idesc_o, (np[i] | part | x) ? 1u : 0u);
+                  const uint32_t k16 = (x >> 1) * 4 + part * 2 + (x & 1);  // a half's probabilities lie in the last 32 of its own 64 columns of scores
+                  umma_f16_ts(tmem + 256 + i * 128, tmem + i * 128 + (x >> 1) * 64 + 32 + (part * 2 + (x & 1)) * 8, v_lo + sv * (UNIT / 16) + k16 * (2048 >> 4),
+                              SMEM_DESC_HI_SW128, idesc_o, (h.made | part | x) ? 1u : 0u);
                 }
               }
             }
             if (leader && ok) {
-              if (t == k.hi[i]) umma_commit(&fin[i]);
+              if (t == h.hi) umma_commit(&fin[i]);
             }
-            ++np[i];
+            ++h.tiles;
+            ++h.made;
           }
-          if (kt && t >= k.lo[i] && t < k.hi[i]) {
+          if (kt && t >= h.lo && t < h.hi) {
             if (!have_k) {
-              if (ok) ok = poll(&full[ik % PT_UNITS], (ik / PT_UNITS) & 1, abort_flag, 940);
+              if (ok) ok = poll(sm + (FULL + sk) * 8, (ik / PT_UNITS) & 1, sm + ABORT, 940);
               have_k = true;
             }
+            if (t == h.lo) {
+              if (ok) ok = poll(sm + (QF + i) * 8, h.loads & 1, sm + ABORT, 910 + i);
+            }
             __syncwarp();
-            scores(i, t);
+            if (leader && ok) {
+              tc_fence_after();
+#pragma unroll
+              for (uint32_t k16 = 0; k16 < DH / 16; ++k16) {
+                umma_f16(tmem + i * 128, q_lo + (i * UNIT + (k16 / 4) * PT_SLAB) / 16 + (k16 & 3) * 2, k_lo + (sk * UNIT + (k16 / 4) * PT_SLAB) / 16 + (k16 & 3) * 2,
+                         SMEM_DESC_HI_SW128, idesc_s, k16 ? 1u : 0u);
+              }
+              umma_commit(&sf[i]);
+            }
           }
-        }
+        };
+        products(std::integral_constant<uint32_t, 0>(), first);
+        products(std::integral_constant<uint32_t, 1>(), second);
         // every tile has a half that uses it, so both units have been waited for
-        if (leader && ok && vt) umma_commit(&empty[iv % PT_UNITS]);
-        if (leader && ok && kt) umma_commit(&empty[ik % PT_UNITS]);
+        if (leader && ok && vt) umma_commit(&empty[sv]);
+        if (leader && ok && kt) umma_commit(&empty[sk]);
       }
-    } else {
-      const uint32_t i = (uint32_t)(warp - 2) >> 3, half = ((uint32_t)(warp - 2) >> 2) & 1, quad = warp & 3, row = quad * 32 + lane;
-      const uint32_t lanes = tmem + (quad * 32 << 16), sb = lanes + i * 128 + half * 64, ob = lanes + 256 + i * 128 + half * (DH / 2);
-      float *mine = meet + (i * 2 + half) * PT_ROWS + row, *theirs = meet + (i * 2 + (half ^ 1)) * PT_ROWS + row;
-      auto meet_other = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + i * 4 + quad) : "memory"); };  // with the other warp of these rows
-      auto agree = [&](bool x) {  // whether any thread of the two warps says so
-        uint32_t any;
-        asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"(1 + i * 4 + quad), "r"((uint32_t)x) : "memory");
-        return any != 0;
+      base += 2 * (t1 - t0);
+      if (ragged) ++tails;
+      auto queries_read = [&](auto I, Half &h) {
+        constexpr uint32_t i = I.value;
+        if (lds(at + offsetof(Segment, k.tokens) + 4 * i)) {
+          // Queries of a half without tiles are waited for all the same: no copy outlives the CTA.
+          if (ok) ok = mbar_wait(&qf[i], h.loads & 1, abort_flag, 912 + i);
+          __syncwarp();
+          ++h.loads;
+          if (lane == 0) arrive(sm + (QE + i) * 8);
+        }
       };
-      const bool live = row < k.tokens[i] * group, any_live = quad * 32 < k.tokens[i] * group;
-      const uint32_t token = k.token0 + i * TT + row / group;
-      const int pos = k.s.pos0 + (int)token;
-      const int lim1 = live ? pos + 1 : 0, lim0 = w.window && pos >= (int)w.window ? pos - (int)w.window + 1 : 0;
-      // tiles that every live row sees whole need no masks
-      const int pos_lo = k.s.pos0 + (int)(k.token0 + i * TT), pos_hi = pos_lo + (int)k.tokens[i] - 1;
-      const int whole0 = w.window ? max(0, pos_hi - (int)w.window + 1) : 0, whole1 = pos_lo + 1;
+      queries_read(std::integral_constant<uint32_t, 0>(), first);
+      queries_read(std::integral_constant<uint32_t, 1>(), second);
+      done();
+    }
+  } else {
+    const uint32_t i = (uint32_t)(warp - 2) >> 3, half = ((uint32_t)(warp - 2) >> 2) & 1, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t lanes = tmem + (quad * 32 << 16), sb = lanes + i * 128 + half * 64, ob = lanes + 256 + i * 128 + half * (DH / 2);
+    const uint32_t mine = sm + MEET + ((i * 2 + half) * PT_ROWS + row) * 4, theirs = sm + MEET + ((i * 2 + (half ^ 1)) * PT_ROWS + row) * 4;
+    auto meet_other = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + i * 4 + quad) : "memory"); };  // with the other warp of these rows
+    auto agree = [&](bool x) {  // whether any thread of the two warps says so
+      uint32_t any;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %2, 0;\n\tbarrier.cta.red.or.pred q, %1, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(any) : "r"(1 + i * 4 + quad), "r"((uint32_t)x) : "memory");
+      return any != 0;
+    };
+    auto meet_all = [] { asm volatile("bar.sync 9, 512;" ::: "memory"); };  // all rows' warps
+    uint8_t *stage = qs + i * UNIT;
+    bool ok = true;
+    uint32_t phases = 0;  // of the half's barriers: 1 scores, 2 ends, 4 queries
+    // Pairs of warps meet in every tile, all of them where blocks are joined.
+    auto together = [&](bool x) {
+      if (!shares) return !agree(!x);
+      uint32_t all;
+      asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 9, 512, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)x) : "memory");
+      return all != 0;
+    };
+    while (const uint32_t g32 = next(ok, together)) {
+      const uint32_t of_half = g32 + i * 4;
+      const uint32_t tokens = lds(of_half + offsetof(Segment, k.tokens)), lo = lds(of_half + offsetof(Segment, k.lo)), n = lds(of_half + offsetof(Segment, k.hi)) - lo;
+      const bool any_live = quad * 32 < tokens * group;
       float m2 = PT_LOWEST, l = 0.f;  // the row's maximum times scale2; the sum of this thread's half
-      bool ok = true;
-      uint32_t n = 0;
-      for (uint32_t t = k.lo[i]; t < k.hi[i]; ++t, ++n) {  // to the end, whatever became of a wait: the two warps of a row meet in every tile
-        if (ok) ok = __all_sync(0xffffffffu, poll(&sf[i], n & 1, abort_flag, 960 + i));
+      // What a tile needs of the segment is read from shared memory where it is needed: the row's scores leave no registers for it.
+      for (uint32_t t = lo; t < lo + n; ++t) {  // to the end, whatever became of a wait: the two warps of a row meet in every tile
+        if (ok) ok = __all_sync(0xffffffffu, poll(sm + (SF + i) * 8, phases & 1, sm + ABORT, 960 + i));
+        phases ^= 1;
         tc_fence_after();
         if (!any_live) {  // rows behind the last: their probabilities may be anything
           if (lane == 0) {
-            mbar_arrive(&pf[2 * i]);
-            mbar_arrive(&pf[2 * i + 1]);
+            arrive(sm + (PF + 2 * i) * 8);
+            arrive(sm + (PF + 2 * i + 1) * 8);
           }
           continue;
         }
-        const int k0 = (int)(t * PT_KEYS);
-        const bool masks = k0 < whole0 || k0 + (int)PT_KEYS > whole1;
-        uint32_t v[2][32];
-        auto hide = [&](int c) {  // scores of keys that the row does not see
+        const bool masks = t < lds(of_half + offsetof(Segment, clear0)) || t >= lds(of_half + offsetof(Segment, clear1));
+        auto hide = [&](uint32_t (&v)[32], int c) {  // scores of keys that the row does not see
           if (masks) {
-            const int a = k0 + (int)half * 64 + c * 32, n0 = min(max(lim0 - a, 0), 32), n1 = min(max(lim1 - a, 0), 32);
+            const int pos = row < tokens * group ? (int)lds(of_half + offsetof(Segment, pos)) + (int)(lds(sm + ROWS + row * 4) & 0xffff) : -1, a = (int)(t * PT_KEYS + half * 64 + c * 32);
+            const int n0 = w.window ? min(max(pos - (int)w.window + 1 - a, 0), 32) : 0, n1 = min(max(pos + 1 - a, 0), 32);
             const uint32_t seen = (uint32_t)((1ull << n1) - 1) & ~(uint32_t)((1ull << n0) - 1);
             if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
 #pragma unroll
               for (int j = 0; j < 32; ++j)
-                if (!(seen >> j & 1)) v[c][j] = 0xFF800000u;
+                if (!(seen >> j & 1)) v[j] = 0xFF800000u;
             }
           }
         };
-        auto largest = [&](int c) {
+        auto largest = [&](const uint32_t (&v)[32]) {
           float tm[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) tm[(j / 2) & 3] = fmaxf(fmaxf(tm[(j / 2) & 3], __uint_as_float(v[c][j])), __uint_as_float(v[c][j + 1]));
+          for (int j = 0; j < 32; j += 2) tm[(j / 2) & 3] = fmaxf(fmaxf(tm[(j / 2) & 3], __uint_as_float(v[j])), __uint_as_float(v[j + 1]));
           return fmaxf(fmaxf(tm[0], tm[1]), fmaxf(tm[2], tm[3]));
         };
-        uint32_t p[16];
-        float sum;
-        auto probabilities = [&](int c) {  // p and their sum
+        // Probabilities of 32 scores into 16 columns of tensor memory, 16 scores at a time; their sum.
+        auto probabilities = [&](const uint32_t (&v)[32], uint32_t to) {
           uint64_t two[2] = {0, 0};
           const uint64_t scale = pair(w.scale2, w.scale2), minus = pair(-m2, -m2);
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            uint64_t x = fma2(pair(__uint_as_float(v[c][2 * j]), __uint_as_float(v[c][2 * j + 1])), scale, minus);
-            if ((j & 3) < PT_EMULATED) {
-              x = exp2_pair(x);
-            } else {
+          for (int h = 0; h < 2; ++h) {
+            uint32_t p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              uint64_t x = fma2(pair(__uint_as_float(v[h * 16 + 2 * j]), __uint_as_float(v[h * 16 + 2 * j + 1])), scale, minus);
+              if ((j & 3) < PT_EMULATED) {
+                x = exp2_pair(x);
+              } else {
+                const float2 f = unpair(x);
+                x = pair(ex2(f.x), ex2(f.y));
+              }
+              two[j & 1] = add2(two[j & 1], x);
               const float2 f = unpair(x);
-              x = pair(ex2(f.x), ex2(f.y));
+              p[j] = pack2<BF16>(f.x, f.y);
             }
-            two[j & 1] = add2(two[j & 1], x);
-            const float2 f = unpair(x);
-            p[j] = pack2<BF16>(f.x, f.y);
+            tmem_st8(to + h * 8, p);
           }
           const float2 s0 = unpair(two[0]), s1 = unpair(two[1]);
-          sum = (s0.x + s0.y) + (s1.x + s1.y);
+          return (s0.x + s0.y) + (s1.x + s1.y);
         };
         auto release = [&](int c) {  // the products of the first 32 keys begin while the others' probabilities are made
-          tmem_st16(sb + c * 16, p);
           tmem_st_wait();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&pf[2 * i + c]);
+          if (lane == 0) arrive(sm + (PF + 2 * i + c) * 8);
         };
-        // The first 32 probabilities are made against the maximum so far, beside the search for the tile's; where it has grown too much (a row's two
-        // threads have to agree, and the barrier tells both) they are made again.
-        tmem_ld32(sb, v[0]);
+        // The first 32 probabilities are made against the maximum so far; where it has grown too much (a row's two threads have to agree, and the barrier tells
+        // both) they are made again, from the scores that still stand: probabilities lie in the columns of the other 32, which are in registers by then.
+        const bool start = t == lo;
+        uint32_t v[32], u[32];
+        tmem_ld32(sb, v);
+        tmem_ld32(sb + 32, u);
         tmem_ld_wait();
-        tmem_ld32(sb + 32, v[1]);
-        hide(0);
-        float tmax = largest(0);
-        probabilities(0);
-        tmem_ld_wait();
-        hide(1);
-        tmax = fmaxf(tmax, largest(1));
-        if (agree(n == 0 || tmax * w.scale2 > m2 + PT_LAZY)) {
-          *mine = tmax;
+        hide(v, 0);
+        hide(u, 1);
+        const float tmax = fmaxf(largest(v), largest(u));
+        float sum = probabilities(v, sb + 32);
+        if (agree(start || tmax * w.scale2 > m2 + PT_LAZY)) {
+          sts(mine, __float_as_uint(tmax));
           meet_other();
-          const float nm = fmaxf(m2, fmaxf(tmax, *theirs) * w.scale2);
-          const bool grown = n == 0 || nm > m2 + PT_LAZY;
+          const float nm = fmaxf(m2, fmaxf(tmax, __uint_as_float(lds(theirs))) * w.scale2);
+          const bool grown = start || nm > m2 + PT_LAZY;
           const float f = grown ? ex2(m2 - nm) : 1.f;
           if (grown) m2 = nm;
           l *= f;
-          if (n) {
+          if (!start) {
 #pragma unroll 1
-            for (uint32_t c = 0; c < DH / 2; c += 16) {
-              tmem_ld16(ob + c, p);
+            for (uint32_t c = 0; c < DH / 2; c += 8) {
+              uint32_t o[8];
+              tmem_ld8(ob + c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int j = 0; j < 16; ++j) p[j] = __float_as_uint(__uint_as_float(p[j]) * f);
-              tmem_st16(ob + c, p);
+              for (int j = 0; j < 8; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+              tmem_st8(ob + c, o);
             }
           }
-          tmem_ld32(sb, v[0]);
+          tmem_ld32(sb, v);
           tmem_ld_wait();
-          hide(0);
-          probabilities(0);
+          hide(v, 0);
+          sum = probabilities(v, sb + 32);
         }
         l += sum;
         release(0);
-        probabilities(1);
-        l += sum;
+        l += probabilities(u, sb + 48);
         release(1);
       }
-      if (ok && n) ok = __all_sync(0xffffffffu, poll(&fin[i], 0, abort_flag, 970 + i));
-      if (any_live) {
-        meet_other();  // the last maximum has been read
-        *mine = l;
-        meet_other();
-        l += *theirs;
+      if (n) {
+        if (ok) ok = __all_sync(0xffffffffu, poll(sm + (FIN + i) * 8, phases >> 1 & 1, sm + ABORT, 970 + i));
+        phases ^= 2;
+      } else if (tokens) {  // no copy of queries meets the outputs there
+        if (ok) ok = __all_sync(0xffffffffu, poll(sm + (QF + i) * 8, phases >> 2 & 1, sm + ABORT, 975 + i));
       }
       if (any_live) {
-        // Outputs go through shared memory (the tile's queries have been used): 16 bytes a lane straight from a row per lane are a line each, and took 5 us
-        // of a block, 6 more until they had drained and the next block could begin.
-        tc_fence_after();
-        uint8_t *stage = qs + i * UNIT;
-        const float inv = m2 == PT_LOWEST ? 0.f : 1.f / l;  // a row that has seen no score: zeros (its sum holds what 2^-126 is for minus infinity)
-        if (ok && n) {
+        meet_other();  // the last maximum has been read
+        sts(mine, __float_as_uint(l));
+        meet_other();
+        l += __uint_as_float(lds(theirs));
+      }
+      tc_fence_after();
+      // Outputs go through shared memory (the half's queries have been used): 16 bytes a lane straight from a row per lane are a line each, and took 5 us
+      // of a block, 6 more until they had drained and the next block could begin.
+      auto put = [&](const float (&y)[32], uint32_t c, float inv) {
+#pragma unroll
+        for (int j = 0; j < 32; j += 8)
+          *reinterpret_cast<uint4 *>(stage + row * (DH * 2) + (((c + j) / 8 ^ (row & 7)) << 4)) =
+              make_uint4(pack2<BF16>(y[j] * inv, y[j + 1] * inv), pack2<BF16>(y[j + 2] * inv, y[j + 3] * inv), pack2<BF16>(y[j + 4] * inv, y[j + 5] * inv),
+                         pack2<BF16>(y[j + 6] * inv, y[j + 7] * inv));
+      };
+      const Segment *g = segments + (had & 1);
+      const uint32_t c0 = g->c0, c1 = g->c1;
+      const bool whole = g->whole;
+      // A part: [maxima][sums][4 elements][row], rows of both halves.
+      auto part_of = [&](uint32_t cta) { return w.parts + (size_t)(2 * cta + (cta == c0 ? 1 : 0)) * PAGED_PART; };
+      const uint32_t r2 = i * PT_ROWS + row;
+      float *own = whole ? nullptr : part_of(blockIdx.x);
+      float inv = m2 == PT_LOWEST ? 0.f : 1.f / l;  // a row that has seen no score: zeros (its sum holds what 2^-126 is for minus infinity)
+      if (any_live) {
 #pragma unroll 1
-          for (uint32_t c = half * (DH / 2); c < (half + 1) * (DH / 2); c += 32) {
+        for (uint32_t c = half * (DH / 2); c < (half + 1) * (DH / 2); c += 32) {
+          float y[32], z = 0.f;  // z: 0, or NaN
+          if (n) {
             uint32_t o[32];
             __syncwarp();
             tmem_ld32(lanes + 256 + i * 128 + c, o);
             tmem_ld_wait();
-            float y[32], z = 0.f;  // z: 0, or NaN
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               y[j] = __uint_as_float(o[j]);
               z = fmaf(y[j], 0.f, z);
             }
-            if (z != 0.f && live && isfinite(l)) {
-              float x[32];  // in memory, which `y` stays out of
+          } else {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) x[j] = y[j];
-              paged_again<32>(w, BF16, false, k.b, k.s, k.g, (k.token0 + i * TT) * group + row, [&](int j) { return c + j; }, max(lim0, (int)(k.lo[i] * PT_KEYS)), lim1, m2, x);
+            for (int j = 0; j < 32; ++j) y[j] = 0.f;
+          }
+          if (z != 0.f && row < tokens * group && isfinite(l)) {
+            const int pos = g->pos[i] + (int)(row / group);
+            float x[32];  // in memory, which `y` stays out of
 #pragma unroll
-              for (int j = 0; j < 32; ++j) y[j] = x[j];
-            }
+            for (int j = 0; j < 32; ++j) x[j] = y[j];
+            paged_again<32>(w, BF16, false, g->b, g->s, g->g, (g->k.token0 + i * TT) * group + row, [&](int j) { return c + j; }, max(w.window ? pos - (int)w.window + 1 : 0, (int)(lo * PT_KEYS)),
+                            min(pos + 1, (int)((lo + n) * PT_KEYS)), m2, x);
 #pragma unroll
-            for (int j = 0; j < 32; j += 8)
-              *reinterpret_cast<uint4 *>(stage + row * (DH * 2) + (((c + j) / 8 ^ (row & 7)) << 4)) =
-                  make_uint4(pack2<BF16>(y[j] * inv, y[j + 1] * inv), pack2<BF16>(y[j + 2] * inv, y[j + 3] * inv), pack2<BF16>(y[j + 4] * inv, y[j + 5] * inv),
-                             pack2<BF16>(y[j + 6] * inv, y[j + 7] * inv));
+            for (int j = 0; j < 32; ++j) y[j] = x[j];
+          }
+          if (whole) {
+            put(y, c, inv);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; j += 4)
+              __stcg(reinterpret_cast<float4 *>(own + 4 * PT_ROWS) + (c + j) / 4 * (2 * PT_ROWS) + r2, make_float4(y[j], y[j + 1], y[j + 2], y[j + 3]));
           }
         }
+      }
+      bool writes = whole;
+      if (!whole) {
+        if (half == 0) {
+          __stcg(own + r2, m2);
+          __stcg(own + 2 * PT_ROWS + r2, l);
+        }
+        __threadfence();
+        meet_all();
+        if (warp == 2 && lane == 0) {
+          const uint32_t before = atomicAdd(w.tickets + c0, 1u);
+          if (before == c1 - c0) w.tickets[c0] = 0;  // all are here: the ticket is free again
+          *ticket = before;
+          __threadfence();
+        }
+        meet_all();
+        writes = *static_cast<volatile uint32_t *>(ticket) == c1 - c0;
+        if (writes && any_live) {  // the last: joins the parts in the order of their tiles
+          float big = PT_LOWEST;
+          for (uint32_t x = c0; x <= c1; ++x) big = fmaxf(big, __ldcg(part_of(x) + r2));
+          l = 0.f;
+          for (uint32_t x = c0; x <= c1; ++x) l = fmaf(__ldcg(part_of(x) + 2 * PT_ROWS + r2), ex2(__ldcg(part_of(x) + r2) - big), l);
+          inv = big == PT_LOWEST ? 0.f : 1.f / l;
+#pragma unroll 1
+          for (uint32_t c = half * (DH / 2); c < (half + 1) * (DH / 2); c += 32) {
+            float y[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) y[j] = 0.f;
+#pragma unroll 1
+            for (uint32_t x = c0; x <= c1; ++x) {
+              const float *from = part_of(x);
+              const float f = ex2(__ldcg(from + r2) - big);
+#pragma unroll
+              for (int j = 0; j < 32; j += 4) {
+                const float4 o = __ldcg(reinterpret_cast<const float4 *>(from + 4 * PT_ROWS) + (c + j) / 4 * (2 * PT_ROWS) + r2);
+                y[j] = fmaf(o.x, f, y[j]);
+                y[j + 1] = fmaf(o.y, f, y[j + 1]);
+                y[j + 2] = fmaf(o.z, f, y[j + 2]);
+                y[j + 3] = fmaf(o.w, f, y[j + 3]);
+              }
+            }
+            put(y, c, inv);
+          }
+        }
+      }
+      if (writes && any_live) {
         meet_other();
         constexpr uint32_t LPR = DH / 8, RPP = 32 / LPR;  // lanes per row, rows per pass
-        const uint32_t e = lane % LPR, rows = k.tokens[i] * group;
+        const uint32_t e = lane % LPR, rows = tokens * group;
+        uint16_t *base = static_cast<uint16_t *>(w.o) + (size_t)(g->s.first + g->k.token0 + i * TT) * w.ld_o + (size_t)g->g * group * w.c.dim;
         if (ok && e * 8 < w.c.dim) {
 #pragma unroll 4
           for (uint32_t x = 0; x < 16; x += RPP) {
             const uint32_t r = quad * 32 + half * 16 + x + lane / LPR;
             if (r >= rows) continue;
-            uint16_t *out = static_cast<uint16_t *>(w.o) + (size_t)(k.s.first + k.token0 + i * TT + r / group) * w.ld_o + (size_t)(k.g * group + r % group) * w.c.dim;
-            *reinterpret_cast<uint4 *>(out + e * 8) = n ? *reinterpret_cast<const uint4 *>(stage + r * (DH * 2) + ((e ^ (r & 7)) << 4)) : make_uint4(0, 0, 0, 0);
+            const uint32_t at = lds(sm + ROWS + r * 4);
+            uint16_t *out = base + (size_t)(at & 0xffff) * w.ld_o + (at >> 16) * w.c.dim;
+            *reinterpret_cast<uint4 *>(out + e * 8) = *reinterpret_cast<const uint4 *>(stage + r * (DH * 2) + ((e ^ (r & 7)) << 4));
           }
         }
       }
+      if (tokens) {
+        phases ^= 4;
+        tc_fence_before();
+        fence_proxy_async();  // what was staged is in front of the queries that take its place
+        __syncwarp();
+        if (lane == 0) arrive(sm + (QE + i) * 8);
+      }
+      done();
     }
   }
   tc_fence_before();
@@ -493,16 +935,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 }
 
 template <int SD, bool BF16>
-int launch_tc(cudaStream_t stream, const PagedAttnArgs &w, uint32_t blocks) {
-  constexpr size_t smem = (size_t)(2 + PT_UNITS) * SD * PT_SLAB + (2 * PT_UNITS + 11) * 8 + 4 * PT_ROWS * 4 + 16;
+int launch_tc(cudaStream_t stream, const PagedAttnArgs &w) {
+  const size_t fixed = (size_t)(2 + PT_UNITS) * SD * PT_SLAB + 1024 + PT_SMALL + 8, per = sizeof(uint64_t) + sizeof(PagedSeq);
   static bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    GRETA_CUDA_TRY(cudaFuncSetAttribute(paged_tc_kernel<SD, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    GRETA_CUDA_TRY(cudaFuncSetAttribute(paged_tc_kernel<SD, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(fixed + PAGED_MAX_BATCH * per)));
     if (dev >= 0 && dev < 64) attr_set[dev] = true;
   }
-  GRETA_CUDA_TRY(launch_pdl(paged_tc_kernel<SD, BF16>, dim3(blocks * w.c.kv_heads), dim3(PT_THREADS), smem, stream, w));
+  const uint32_t grid = std::min<uint32_t>(PT_MAX_CTAS, sm_count());  // one a SM: its tensor memory and most of its shared memory
+  GRETA_CUDA_TRY(launch_pdl(paged_tc_kernel<SD, BF16>, dim3(grid), dim3(PT_THREADS), fixed + w.r.batch * per, stream, w));
   return launched("paged_tc_kernel");
 }
 
@@ -523,10 +966,10 @@ int paged_attn_tc(cudaStream_t stream, PagedAttnArgs &w, uint32_t heads) {
     set_error("paged_attn: cuTensorMapEncodeTiled failed with code %d", (int)r);
     return GRETA_ERR_INVALID_ARGS;
   }
-  const uint32_t blocks = w.r.tokens / (2 * TT) + std::min(w.r.batch, w.r.tokens);  // no sequence has more than its whole blocks and one
-  GRETA_REQUIRE((uint64_t)blocks * w.c.kv_heads < (1ull << 31), "paged_attn: %u blocks of %u heads", blocks, w.c.kv_heads);
-  if (d > 64) return bf16 ? launch_tc<2, true>(stream, w, blocks) : launch_tc<2, false>(stream, w, blocks);
-  return bf16 ? launch_tc<1, true>(stream, w, blocks) : launch_tc<1, false>(stream, w, blocks);
+  // Numbers of blocks, and places of a sequence (48 bits) with them, fit their words.
+  GRETA_REQUIRE((uint64_t)(w.r.tokens / (2 * TT) + w.r.batch) * w.c.kv_heads < (1ull << 31) && w.r.tokens / (2 * TT) < 65535, "paged_attn: %u rows of %u heads", w.r.tokens, heads);
+  if (d > 64) return bf16 ? launch_tc<2, true>(stream, w) : launch_tc<2, false>(stream, w);
+  return bf16 ? launch_tc<1, true>(stream, w) : launch_tc<1, false>(stream, w);
 }
 
 }  // namespace greta
