@@ -29,7 +29,6 @@ constexpr uint32_t PT_JOIN = 6;    // what joining the shares' parts costs, in t
 constexpr uint32_t PT_MAX_CTAS = PAGED_TC_CTAS;
 constexpr uint32_t PT_BARRIERS = 28, PT_SMALL = 3328;  // of a CTA; bytes of shared memory for them, exchanges, segments and words
 constexpr uint32_t PT_SLAB = 128 * 128;  // bytes of 64 elements of 128 rows
-constexpr int PT_EMULATED = 1;           // pairs of probabilities out of four that the FMA units make: the special-function unit's 16 a clock bound the tile otherwise
 constexpr float PT_LAZY = 8.f;           // log2 of what a row's maximum may grow by before its sums are rescaled
 constexpr float PT_LOWEST = -3.4028234e38f;  // a row's maximum before any score
 
@@ -80,9 +79,7 @@ __device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity, uint32_t abo
   } while (!ok && !lds(abort_flag));
   return ok;
 }
-__device__ __forceinline__ bool poll(uint64_t *bar, uint32_t parity, volatile int *abort_flag, int code) {
-  return poll(smem_u32(bar), parity, smem_u32(const_cast<int *>(abort_flag)), code);
-}
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t abort_flag, int code) { return poll(bar, parity, abort_flag, code); }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if (!BF16) return half2_bits(a, b);
@@ -122,20 +119,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^x of two values without the special-function unit: x = n + r, n an integer (by adding 1.5 * 2^23, whose last place is one) and |r| <= 1/2; a polynomial in r of
-// degree 3, fitted to the smallest largest relative error over that interval (7.5e-5, a quarter of half a step of fp16); n is added to its exponent.
-__device__ __forceinline__ uint64_t exp2_pair(uint64_t x) {
-  const uint64_t big = pair(12582912.f, 12582912.f);
-  const float2 f = unpair(x);
-  x = pair(fmaxf(f.x, -126.f), fmaxf(f.y, -126.f));
-  const uint64_t t = add2(x, big), n = add2(t, pair(-12582912.f, -12582912.f)), r = fma2(n, pair(-1.f, -1.f), x);
-  uint64_t p = fma2(r, pair(0.0551716685f, 0.0551716685f), pair(0.242611125f, 0.242611125f));
-  p = fma2(p, r, pair(0.693260968f, 0.693260968f));
-  p = fma2(p, r, pair(0.999928057f, 0.999928057f));
-  const float2 y = unpair(p), e = unpair(t);
-  return pair(__int_as_float(__float_as_int(y.x) + (__float_as_int(e.x) << 23)), __int_as_float(__float_as_int(y.y) + (__float_as_int(e.y) << 23)));
-}
-
 // A block of rows of one sequence and KV head: its tokens as two halves, and the key tiles lo .. hi - 1 that each sees; t0 .. t1 - 1 is both.
 struct Block {
   uint32_t token0, tokens[2], lo[2], hi[2], t0, t1;
@@ -296,17 +279,17 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
   constexpr uint32_t DH = SD * 64, UNIT = SD * PT_SLAB;
   extern __shared__ uint8_t smem_raw[];
   uint8_t *smem = reinterpret_cast<uint8_t *>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint8_t *qs = smem, *ring = qs + 2 * UNIT;  // queries of both halves, then their outputs; keys and values in turn
-  uint64_t *bars = reinterpret_cast<uint64_t *>(ring + PT_UNITS * UNIT);
-  constexpr uint32_t FULL = 0, EMPTY = FULL + PT_UNITS, QF = EMPTY + PT_UNITS, QE = QF + 2, SF = QE + 2, PF = SF + 2, FIN = PF + 4, VL = FIN + 2, VZ = VL + 1, NF = VZ + 2, NE = NF + 2;
-  static_assert(NE + 2 <= PT_BARRIERS, "barriers");
-  uint64_t *full = bars + FULL, *empty = bars + EMPTY, *qf = bars + QF, *qe = bars + QE, *sf = bars + SF, *pf = bars + PF, *fin = bars + FIN;
-  uint64_t *vl = bars + VL, *vz = bars + VZ;  // the last values of a ragged sequence have come; and hold zeros behind its end (two in turn: one may follow the other at once)
-  uint64_t *nf = bars + NF, *ne = bars + NE;  // the next segment is there; is done with
-  // Behind the barriers: [half][column half][row] floats that the two threads of a row tell each other; [row] its token and head (divisions by the group,
-  // once); two segments (warp 0 finds them, one ahead; the others leave in them what they need late); words; and what depends on the batch.
-  constexpr uint32_t MEET = PT_BARRIERS * 8, ROWS = MEET + 4 * PT_ROWS * 4, SEGMENTS = ROWS + PT_ROWS * 4, WORDS = SEGMENTS + 2 * sizeof(Segment);
-  uint8_t *small = reinterpret_cast<uint8_t *>(bars);
+  uint8_t *qs = smem, *ring = qs + 2 * UNIT;  // queries of both halves; keys and values in turn
+  uint8_t *small = ring + PT_UNITS * UNIT;
+  constexpr uint32_t MEET = 0, BARS = 4 * PT_ROWS * 4;  // [half][column half][row] floats that the two threads of a row tell each other (512 bytes apart); barriers
+  constexpr uint32_t FULL = BARS / 8, EMPTY = FULL + PT_UNITS, QF = EMPTY + PT_UNITS, QE = QF + 2, SF = QE + 2, PF = SF + 2, FIN = PF + 4, VL = FIN + 2, VZ = VL + 1, NF = VZ + 2, NE = NF + 2;
+  static_assert(NE + 2 <= BARS / 8 + PT_BARRIERS, "barriers");
+  uint64_t *all = reinterpret_cast<uint64_t *>(small), *full = all + FULL, *empty = all + EMPTY, *qf = all + QF, *qe = all + QE, *sf = all + SF, *pf = all + PF, *fin = all + FIN;
+  uint64_t *vl = all + VL, *vz = all + VZ;  // the last values of a ragged sequence have come; and hold zeros behind its end (two in turn: one may follow the other at once)
+  uint64_t *nf = all + NF, *ne = all + NE;  // the next segment is there; is done with
+  // Behind the barriers: [row] its token and head (divisions by the group, once); two segments (warp 0 finds them, one ahead; the others leave in them what they
+  // need late); words; and what depends on the batch.
+  constexpr uint32_t ROWS = BARS + PT_BARRIERS * 8, SEGMENTS = ROWS + PT_ROWS * 4, WORDS = SEGMENTS + 2 * sizeof(Segment);
   Segment *segments = reinterpret_cast<Segment *>(small + SEGMENTS);
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(small + WORDS), *ticket = tmem_slot + 1, *limits = ticket + 1;  // limits: cost of the largest and of the smallest block
   volatile int *abort_flag = reinterpret_cast<volatile int *>(limits + 2);
@@ -314,7 +297,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
   uint64_t *prefix = reinterpret_cast<uint64_t *>(small + PT_SMALL);  // [batch + 1]: places (or blocks) in front of a sequence
   PagedSeq *seqs = reinterpret_cast<PagedSeq *>(prefix + w.r.batch + 1);
   static_assert(WORDS + 32 <= PT_SMALL, "small things");
-  const uint32_t sm = smem_u32(bars);
+  const uint32_t sm = smem_u32(small);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const uint32_t group = w.group, TT = PT_ROWS / group, G = w.c.kv_heads, N = gridDim.x;
 
@@ -325,7 +308,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&qf[i], 1);
-      mbar_init(&qe[i], 9);  // the half's warps, and the one that issues
+      mbar_init(&qe[i], 1);
       mbar_init(&sf[i], 1);
       mbar_init(&pf[2 * i], 8);  // the first and the second 32 keys of both warps of a row
       mbar_init(&pf[2 * i + 1], 8);
@@ -456,7 +439,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         more = id < total;
         if (more) find.block(id, g);
       }
-      if (ok) ok = poll(&ne[x], (handed >> 1 & 1) ^ 1, abort_flag, 985);
+      if (ok) ok = poll(sm + (NE + x) * 8, (handed >> 1 & 1) ^ 1, sm + ABORT, 985);
       ++handed;
       __syncwarp();
       if (lane == 0) {
@@ -471,7 +454,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
       const uint32_t p = t * PT_KEYS + lane * box;
       return lane < boxes && t < end && p < g->s.len ? __ldcg(w.c.table + (size_t)g->b * w.c.ld_table + p / w.c.page) : -1;
     };
-    // Queries of the two halves take the place of the block before's outputs, each when those have left; the copies of keys and values do not wait for that.
+    // Queries of the two halves take the place of the block before's, each when its last scores have been made; the copies of keys and values do not wait for that.
     const Segment *asking = nullptr;
     uint32_t asked = 0;  // bits: halves whose queries have been asked for
     auto ask = [&](uint32_t i, uint32_t &loads) {
@@ -510,7 +493,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     uint32_t tail_at = 0, tail_from = PT_KEYS;  // the unit with a ragged sequence's last values, and where its zeros begin
     auto zeros = [&] {
       if (tail_from < PT_KEYS) {
-        if (ok) ok = mbar_wait(vl, tails & 1, abort_flag, 950);
+        if (ok) ok = mbar_wait(sm + VL * 8, tails & 1, sm + ABORT, 950);
         __syncwarp();
         ++tails;
         if (ok) {
@@ -635,6 +618,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
                          SMEM_DESC_HI_SW128, idesc_s, k16 ? 1u : 0u);
               }
               umma_commit(&sf[i]);
+              if (t + 1 == h.hi) umma_commit(&qe[i]);
             }
           }
         };
@@ -650,10 +634,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         constexpr uint32_t i = I.value;
         if (lds(at + offsetof(Segment, k.tokens) + 4 * i)) {
           // Queries of a half without tiles are waited for all the same: no copy outlives the CTA.
-          if (ok) ok = mbar_wait(&qf[i], h.loads & 1, abort_flag, 912 + i);
-          __syncwarp();
+          if (h.lo == h.hi) {
+            if (ok) ok = mbar_wait(sm + (QF + i) * 8, h.loads & 1, sm + ABORT, 912 + i);
+            __syncwarp();
+            if (lane == 0) arrive(sm + (QE + i) * 8);
+          }
           ++h.loads;
-          if (lane == 0) arrive(sm + (QE + i) * 8);
         }
       };
       queries_read(std::integral_constant<uint32_t, 0>(), first);
@@ -662,8 +648,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     }
   } else {
     const uint32_t i = (uint32_t)(warp - 2) >> 3, half = ((uint32_t)(warp - 2) >> 2) & 1, quad = warp & 3, row = quad * 32 + lane;
-    const uint32_t lanes = tmem + (quad * 32 << 16), sb = lanes + i * 128 + half * 64, ob = lanes + 256 + i * 128 + half * (DH / 2);
-    const uint32_t mine = sm + MEET + ((i * 2 + half) * PT_ROWS + row) * 4, theirs = sm + MEET + ((i * 2 + (half ^ 1)) * PT_ROWS + row) * 4;
+    const uint32_t sb = tmem + (quad * 32 << 16) + i * 128 + half * 64, ob = sb + 256 - half * (64 - DH / 2);  // the thread's scores, and outputs
+    const uint32_t mine = sm + MEET + ((i * 2 + half) * PT_ROWS + row) * 4, theirs = mine ^ (PT_ROWS * 4);
     auto meet_other = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + i * 4 + quad) : "memory"); };  // with the other warp of these rows
     auto agree = [&](bool x) {  // whether any thread of the two warps says so
       uint32_t any;
@@ -671,12 +657,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
       return any != 0;
     };
     auto meet_all = [] { asm volatile("bar.sync 9, 512;" ::: "memory"); };  // all rows' warps
-    uint8_t *stage = qs + i * UNIT;
     bool ok = true;
-    uint32_t phases = 0;  // of the half's barriers: 1 scores, 2 ends, 4 queries
+    uint32_t phases = 0;  // of the half's barriers: 1 scores, 2 ends
     // Pairs of warps meet in every tile, all of them where blocks are joined.
     auto together = [&](bool x) {
-      if (!shares) return !agree(!x);
+      if (!lds(sm + WORDS + 8)) return !agree(!x);  // no shares
       uint32_t all;
       asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, 9, 512, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)x) : "memory");
       return all != 0;
@@ -726,16 +711,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             uint32_t p[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              uint64_t x = fma2(pair(__uint_as_float(v[h * 16 + 2 * j]), __uint_as_float(v[h * 16 + 2 * j + 1])), scale, minus);
-              if ((j & 3) < PT_EMULATED) {
-                x = exp2_pair(x);
-              } else {
-                const float2 f = unpair(x);
-                x = pair(ex2(f.x), ex2(f.y));
-              }
-              two[j & 1] = add2(two[j & 1], x);
-              const float2 f = unpair(x);
-              p[j] = pack2<BF16>(f.x, f.y);
+              const float2 x = unpair(fma2(pair(__uint_as_float(v[h * 16 + 2 * j]), __uint_as_float(v[h * 16 + 2 * j + 1])), scale, minus));
+              const float a = ex2(x.x), b = ex2(x.y);
+              two[j & 1] = add2(two[j & 1], pair(a, b));
+              p[j] = pack2<BF16>(a, b);
             }
             tmem_st8(to + h * 8, p);
           }
@@ -791,8 +770,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
       if (n) {
         if (ok) ok = __all_sync(0xffffffffu, poll(sm + (FIN + i) * 8, phases >> 1 & 1, sm + ABORT, 970 + i));
         phases ^= 2;
-      } else if (tokens) {  // no copy of queries meets the outputs there
-        if (ok) ok = __all_sync(0xffffffffu, poll(sm + (QF + i) * 8, phases >> 2 & 1, sm + ABORT, 975 + i));
       }
       if (any_live) {
         meet_other();  // the last maximum has been read
@@ -801,23 +778,46 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         l += __uint_as_float(lds(theirs));
       }
       tc_fence_after();
-      // Outputs go through shared memory (the half's queries have been used): 16 bytes a lane straight from a row per lane are a line each, and took 5 us
-      // of a block, 6 more until they had drained and the next block could begin.
-      auto put = [&](const float (&y)[32], uint32_t c, float inv) {
-#pragma unroll
-        for (int j = 0; j < 32; j += 8)
-          *reinterpret_cast<uint4 *>(stage + row * (DH * 2) + (((c + j) / 8 ^ (row & 7)) << 4)) =
-              make_uint4(pack2<BF16>(y[j] * inv, y[j + 1] * inv), pack2<BF16>(y[j + 2] * inv, y[j + 3] * inv), pack2<BF16>(y[j + 4] * inv, y[j + 5] * inv),
-                         pack2<BF16>(y[j + 6] * inv, y[j + 7] * inv));
-      };
       const Segment *g = segments + (had & 1);
       const uint32_t c0 = g->c0, c1 = g->c1;
       const bool whole = g->whole;
+      // 32 elements of the thread's row from c on, as they are stored.  16 bytes a lane straight from a row per lane would be a line each: four lanes change places
+      // (a 4 x 4 transposition of 16-byte pieces), and store 64 bytes of each of their rows in turn.
+      uint16_t *base = static_cast<uint16_t *>(w.o) + (size_t)(g->s.first + g->k.token0 + i * TT) * w.ld_o + (size_t)g->g * group * w.c.dim;
+      auto put = [&](const float (&y)[32], uint32_t c, float inv) {
+        __syncwarp();
+        uint32_t q[4][4];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) q[j / 4][j & 3] = pack2<BF16>(y[2 * j] * inv, y[2 * j + 1] * inv);
+#pragma unroll
+        for (int s = 1; s < 4; s *= 2)
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (!(x & s)) {
+              const bool up = lane & s;
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? q[x][j] : q[x + s][j], s);
+                if (up)
+                  q[x][j] = got;
+                else
+                  q[x + s][j] = got;
+              }
+            }
+        const uint32_t e = c + (lane & 3) * 8;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t r = (row & ~3u) + x;
+          if (r >= tokens * group || e >= w.c.dim || !ok) continue;
+          const uint32_t at = lds(sm + ROWS + r * 4);
+          *reinterpret_cast<uint4 *>(base + (size_t)(at & 0xffff) * w.ld_o + (at >> 16) * w.c.dim + e) = make_uint4(q[x][0], q[x][1], q[x][2], q[x][3]);
+        }
+      };
       // A part: [maxima][sums][4 elements][row], rows of both halves.
       auto part_of = [&](uint32_t cta) { return w.parts + (size_t)(2 * cta + (cta == c0 ? 1 : 0)) * PAGED_PART; };
       const uint32_t r2 = i * PT_ROWS + row;
       float *own = whole ? nullptr : part_of(blockIdx.x);
-      float inv = m2 == PT_LOWEST ? 0.f : 1.f / l;  // a row that has seen no score: zeros (its sum holds what 2^-126 is for minus infinity)
+      float inv = m2 == PT_LOWEST ? 0.f : 1.f / l;  // a row that has seen no score: zeros
       if (any_live) {
 #pragma unroll 1
         for (uint32_t c = half * (DH / 2); c < (half + 1) * (DH / 2); c += 32) {
@@ -825,7 +825,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
           if (n) {
             uint32_t o[32];
             __syncwarp();
-            tmem_ld32(lanes + 256 + i * 128 + c, o);
+            tmem_ld32(ob + c - half * (DH / 2), o);
             tmem_ld_wait();
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
@@ -855,7 +855,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
           }
         }
       }
-      bool writes = whole;
       if (!whole) {
         if (half == 0) {
           __stcg(own + r2, m2);
@@ -870,8 +869,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
           __threadfence();
         }
         meet_all();
-        writes = *static_cast<volatile uint32_t *>(ticket) == c1 - c0;
-        if (writes && any_live) {  // the last: joins the parts in the order of their tiles
+        if (lds(sm + WORDS + 4) == c1 - c0 && any_live) {  // the last: joins the parts in the order of their tiles
           float big = PT_LOWEST;
           for (uint32_t x = c0; x <= c1; ++x) big = fmaxf(big, __ldcg(part_of(x) + r2));
           l = 0.f;
@@ -899,29 +897,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
           }
         }
       }
-      if (writes && any_live) {
-        meet_other();
-        constexpr uint32_t LPR = DH / 8, RPP = 32 / LPR;  // lanes per row, rows per pass
-        const uint32_t e = lane % LPR, rows = tokens * group;
-        uint16_t *base = static_cast<uint16_t *>(w.o) + (size_t)(g->s.first + g->k.token0 + i * TT) * w.ld_o + (size_t)g->g * group * w.c.dim;
-        if (ok && e * 8 < w.c.dim) {
-#pragma unroll 4
-          for (uint32_t x = 0; x < 16; x += RPP) {
-            const uint32_t r = quad * 32 + half * 16 + x + lane / LPR;
-            if (r >= rows) continue;
-            const uint32_t at = lds(sm + ROWS + r * 4);
-            uint16_t *out = base + (size_t)(at & 0xffff) * w.ld_o + (at >> 16) * w.c.dim;
-            *reinterpret_cast<uint4 *>(out + e * 8) = *reinterpret_cast<const uint4 *>(stage + r * (DH * 2) + ((e ^ (r & 7)) << 4));
-          }
-        }
-      }
-      if (tokens) {
-        phases ^= 4;
-        tc_fence_before();
-        fence_proxy_async();  // what was staged is in front of the queries that take its place
-        __syncwarp();
-        if (lane == 0) arrive(sm + (QE + i) * 8);
-      }
+      tc_fence_before();  // the outputs have been read: the next products may take their place
       done();
     }
   }
