@@ -3,7 +3,7 @@
 // A CTA takes a block of 256 query rows of one KV head as two tiles of 128: row R of a sequence and KV head is token R / group, head R % group, so a tile
 // is 128 / group tokens with all their heads and every key tile is fetched once for them.  Keys come in tiles of 128, page by page, by TMA (a page's rows of a head
 // are contiguous); queries by TMA as boxes of [tokens][group][64].
-//   warp 0: copies, and zeros over what the last page holds behind the sequence's end; warp 1: MMAs; warps 2-9 and 10-17: the rows of the first and
+//   warp 0: copies; warp 1: MMAs; warps 2-9 and 10-17: the rows of the first and
 //   second tile, two threads each (64 keys of a tile, half of the outputs): maxima, probabilities, outputs.
 // The two tiles take turns: while the tensor core multiplies one (P V of this key tile, Q K of the next), the other's probabilities are made.
 //   tensor memory: scores of tile A and B at columns 0 and 128, each half of which is overwritten by its probabilities (32 columns), outputs at 256 and 384.
@@ -24,8 +24,8 @@ using namespace greta;
 namespace {
 
 constexpr uint32_t PT_ROWS = 128, PT_KEYS = 128, PT_THREADS = 576, PT_UNITS = 4, PT_TMEM = 512;
-constexpr uint32_t PT_LIST = 3;    // what a block costs besides its key tiles, in tiles: its queries, sums and outputs
-constexpr uint32_t PT_JOIN = 6;    // what joining the shares' parts costs, in tiles
+constexpr uint32_t PT_TILE1 = 6, PT_TILE2 = 6, PT_LIST1 = 10, PT_LIST2 = 18;  // places of a key tile and of a block's beginning and end, with one half and with two
+constexpr uint32_t PT_JOIN = 32;                                               // what joining the shares' parts costs
 constexpr uint32_t PT_MAX_CTAS = PAGED_TC_CTAS;
 constexpr uint32_t PT_BARRIERS = 28, PT_SMALL = 3328;  // of a CTA; bytes of shared memory for them, exchanges, segments and words
 constexpr uint32_t PT_SLAB = 128 * 128;  // bytes of 64 elements of 128 rows
@@ -140,15 +140,18 @@ __device__ __forceinline__ Block block_of(const PagedSeq &s, uint32_t j, uint32_
   k.t1 = max(k.hi[0], k.hi[1]);
   return k;
 }
-// What a block costs: its tiles (one where it sees no key) and PT_LIST for its beginning and end.
-__device__ __forceinline__ uint32_t places_of(const Block &k) { return max(1u, k.t1 - k.t0) + PT_LIST; }
+// What a block costs, in places of about 0.3 us: a key tile of two halves, or of one (whose tensor core and special-function unit wait for each other), and its beginning
+// and end.  The tiles of a block that sees no key are taken for one.
+__device__ __forceinline__ uint32_t tile_places(const Block &k) { return k.tokens[1] ? PT_TILE2 : PT_TILE1; }
+__device__ __forceinline__ uint32_t list_places(const Block &k) { return k.tokens[1] ? PT_LIST2 : PT_LIST1; }
+__device__ __forceinline__ uint32_t places_of(const Block &k) { return max(1u, k.t1 - k.t0) * tile_places(k) + list_places(k); }
 
 // What a CTA works on at a time: a block of a KV head, its tiles clipped to k.t0 .. k.t1 - 1.
 struct Segment {
   Block k;
   PagedSeq s;
   uint32_t b, g;
-  uint32_t whole, ragged;  // all of the block; the last tile is the last of the sequence and holds rows behind its end
+  uint32_t whole, tail;    // all of the block; rows of the last tile that lie behind the sequence's end
   uint32_t c0, c1;         // the CTAs that share the block
   uint32_t clear0[2], clear1[2];  // of a half: the tiles that all its rows see whole
   int pos[2];              // of a half: its first row's position
@@ -158,21 +161,21 @@ struct Segment {
 // What is to be done, in the order of its places: sequences, their blocks from the last (and longest) to the first, KV heads.  Used by all lanes of a warp.
 struct Finder {
   const PagedAttnArgs &w;
-  const uint64_t *prefix;  // places (or blocks) in front of a sequence, and of the end
+  const uint32_t *prefix;  // places (or blocks) in front of a sequence, and of the end
   const PagedSeq *seqs;
-  const uint64_t share;    // places of each CTA
+  const uint32_t share;    // places of each CTA
   const uint32_t TT, G, lane;
-  uint64_t at, stop, begin = 0;  // the next place, the end of the CTA's; the first place of the block that `at` lies in
+  uint32_t at, stop, begin = 0;  // the next place, the end of the CTA's; the first place of the block that `at` lies in
   uint32_t cur = 0, jj = 0, kvh = 0;  // that block: sequence, number from the last, KV head
   bool found = false;
 
-  __device__ Finder(const PagedAttnArgs &w, const uint64_t *prefix, const PagedSeq *seqs, uint64_t share)
+  __device__ Finder(const PagedAttnArgs &w, const uint32_t *prefix, const PagedSeq *seqs, uint32_t share)
       : w(w), prefix(prefix), seqs(seqs), share(share), TT(PT_ROWS / w.group), G(w.c.kv_heads), lane(threadIdx.x & 31) {
     at = min(prefix[w.r.batch], share * blockIdx.x);
     stop = min(prefix[w.r.batch], at + share);
   }
   __device__ uint32_t blocks_of(const PagedSeq &s) const { return (s.rows + 2 * TT - 1) / (2 * TT); }
-  __device__ uint32_t seq_at(uint64_t x) const {  // prefix[b] <= x < prefix[b + 1]
+  __device__ uint32_t seq_at(uint32_t x) const {  // prefix[b] <= x < prefix[b + 1]
     uint32_t lo = 0, hi = w.r.batch;
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
@@ -193,23 +196,23 @@ struct Finder {
       g.clear1[i] = first < 0 ? 0 : (uint32_t)(first + 1) / PT_KEYS;
     }
   }
-  __device__ bool ragged(const Segment &g) const { return g.k.t1 > g.k.t0 && (int)(g.k.t1 * PT_KEYS) > g.s.pos0 + (int)g.s.rows; }
+  __device__ uint32_t tail(const Segment &g) const { return g.k.t1 > g.k.t0 ? (uint32_t)max(0, (int)(g.k.t1 * PT_KEYS) - (g.s.pos0 + (int)g.s.rows)) : 0; }
   // A whole block by its number.
   __device__ void block(uint32_t x, Segment &g) const {
     g.b = seq_at(x);
     g.s = seqs[g.b];
-    const uint32_t in = x - (uint32_t)prefix[g.b];
+    const uint32_t in = x - prefix[g.b];
     g.g = in % G;
     g.k = block_of(g.s, blocks_of(g.s) - 1 - in / G, TT, w.window);
     g.c0 = g.c1 = 0;
-    g.ragged = ragged(g);
+    g.tail = tail(g);
     finish(g);
   }
   __device__ void search() {  // the share's beginning: which sequence, and which of its blocks, 32 at a time
     cur = seq_at(at);
     const PagedSeq s = seqs[cur];
     const uint32_t blocks = blocks_of(s);
-    uint64_t before = prefix[cur];
+    uint32_t before = prefix[cur];
     for (uint32_t j0 = 0; !found; j0 += 32) {
       const uint32_t mine = j0 + lane < blocks ? places_of(block_of(s, blocks - 1 - j0 - lane, TT, w.window)) * G : 0;
       uint32_t v = mine;
@@ -224,8 +227,8 @@ struct Finder {
         const int l = hit ? __ffs(hit) - 1 : 0;
         jj = j0 + l;
         const uint32_t first = __shfl_sync(0xffffffffu, v - mine, l), each = __shfl_sync(0xffffffffu, mine, l) / G;
-        kvh = (uint32_t)((at - before - first) / each);
-        begin = before + first + (uint64_t)kvh * each;
+        kvh = (at - before - first) / each;
+        begin = before + first + kvh * each;
       }
       before += __shfl_sync(0xffffffffu, v, 31);
     }
@@ -239,8 +242,11 @@ struct Finder {
       g.s = seqs[cur];
       const uint32_t blocks = blocks_of(g.s);
       g.k = block_of(g.s, blocks - 1 - jj, TT, w.window);
-      const uint32_t tiles = g.k.t1 - g.k.t0, places = places_of(g.k), p = (uint32_t)(at - begin), n = (uint32_t)min((uint64_t)(places - p), stop - at);
-      const uint64_t first = begin + PT_LIST, end = begin + places;
+      const uint32_t tiles = g.k.t1 - g.k.t0, places = places_of(g.k), p = at - begin, n = min(places - p, stop - at);
+      // A tile is the CTA's that its first place falls to.
+      const uint32_t each = tile_places(g.k), list = list_places(g.k), end = begin + places;
+      auto tile_at = [&](uint32_t x) { return x <= list ? 0 : (x - list + each - 1) / each; };
+      const uint32_t a = tile_at(p), z = tile_at(p + n), c0 = (begin + list) / share, c1 = (end - each) / share;
       at += n;
       if (at == end) {  // on to the next block
         begin = end;
@@ -253,10 +259,9 @@ struct Finder {
           }
         }
       }
-      const uint32_t a = max(p, PT_LIST) - PT_LIST, z = max(p + n, PT_LIST) - PT_LIST;
       if (a == z) continue;
-      g.c0 = (uint32_t)(first / share);
-      g.c1 = (uint32_t)((end - 1) / share);
+      g.c0 = c0;
+      g.c1 = c1;
       const uint32_t t0 = g.k.t0 + min(a, tiles), t1 = g.k.t0 + min(z, tiles);
       const bool to_end = t1 == g.k.t1;
       g.k.t0 = t0;
@@ -266,7 +271,7 @@ struct Finder {
         g.k.lo[i] = min(max(g.k.lo[i], t0), t1);
         g.k.hi[i] = max(min(g.k.hi[i], t1), g.k.lo[i]);
       }
-      g.ragged = to_end && ragged(g);
+      g.tail = to_end ? tail(g) : 0;
       finish(g);
       return true;
     }
@@ -282,10 +287,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
   uint8_t *qs = smem, *ring = qs + 2 * UNIT;  // queries of both halves; keys and values in turn
   uint8_t *small = ring + PT_UNITS * UNIT;
   constexpr uint32_t MEET = 0, BARS = 4 * PT_ROWS * 4;  // [half][column half][row] floats that the two threads of a row tell each other (512 bytes apart); barriers
-  constexpr uint32_t FULL = BARS / 8, EMPTY = FULL + PT_UNITS, QF = EMPTY + PT_UNITS, QE = QF + 2, SF = QE + 2, PF = SF + 2, FIN = PF + 4, VL = FIN + 2, VZ = VL + 1, NF = VZ + 2, NE = NF + 2;
+  constexpr uint32_t FULL = BARS / 8, EMPTY = FULL + PT_UNITS, QF = EMPTY + PT_UNITS, QE = QF + 2, SF = QE + 2, PF = SF + 2, FIN = PF + 4, NF = FIN + 2, NE = NF + 2;
   static_assert(NE + 2 <= BARS / 8 + PT_BARRIERS, "barriers");
   uint64_t *all = reinterpret_cast<uint64_t *>(small), *full = all + FULL, *empty = all + EMPTY, *qf = all + QF, *qe = all + QE, *sf = all + SF, *pf = all + PF, *fin = all + FIN;
-  uint64_t *vl = all + VL, *vz = all + VZ;  // the last values of a ragged sequence have come; and hold zeros behind its end (two in turn: one may follow the other at once)
   uint64_t *nf = all + NF, *ne = all + NE;  // the next segment is there; is done with
   // Behind the barriers: [row] its token and head (divisions by the group, once); two segments (warp 0 finds them, one ahead; the others leave in them what they
   // need late); words; and what depends on the batch.
@@ -294,8 +298,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
   uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(small + WORDS), *ticket = tmem_slot + 1, *limits = ticket + 1;  // limits: cost of the largest and of the smallest block
   volatile int *abort_flag = reinterpret_cast<volatile int *>(limits + 2);
   constexpr uint32_t ABORT = WORDS + 16;
-  uint64_t *prefix = reinterpret_cast<uint64_t *>(small + PT_SMALL);  // [batch + 1]: places (or blocks) in front of a sequence
-  PagedSeq *seqs = reinterpret_cast<PagedSeq *>(prefix + w.r.batch + 1);
+  uint32_t *prefix = reinterpret_cast<uint32_t *>(small + PT_SMALL);  // [batch + 1]: places (or blocks) in front of a sequence; and [batch] its blocks
+  uint32_t *blocks_in = prefix + w.r.batch + 1;
+  PagedSeq *seqs = reinterpret_cast<PagedSeq *>(blocks_in + w.r.batch);
   static_assert(WORDS + 32 <= PT_SMALL, "small things");
   const uint32_t sm = smem_u32(small);
   const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -316,9 +321,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
       mbar_init(&nf[i], 1);
       mbar_init(&ne[i], 17);
     }
-    mbar_init(vl, 1);
-    mbar_init(vz, 1);
-    mbar_init(vz + 1, 1);
     limits[0] = 0;
     limits[1] = 0xffffffffu;
     *abort_flag = 0;
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
   for (uint32_t b = warp; b < w.r.batch; b += PT_THREADS / 32) {
     const PagedSeq s = seqs[b];
     const uint32_t blocks = (s.rows + 2 * TT - 1) / (2 * TT);
-    uint32_t sum = 0, most = 0, least = 0xffffffffu;  // places of 2^24 rows' blocks over 2^24 tiles each would not fit, in 32 bits; nor would the work end
+    uint32_t sum = 0, most = 0, least = 0xffffffffu;
     for (uint32_t j = lane; j < blocks; j += 32) {
       const uint32_t n = places_of(block_of(s, j, TT, w.window));
       sum += n;
@@ -358,34 +360,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     most = __reduce_max_sync(0xffffffffu, most);
     least = __reduce_min_sync(0xffffffffu, least);
     if (lane == 0) {
-      prefix[b + 1] = (uint64_t)all * G | (uint64_t)blocks << 48;
+      prefix[b + 1] = all * G;
+      blocks_in[b] = blocks;
       atomicMax(&limits[0], most);
       atomicMin(&limits[1], least);
     }
   }
   __syncthreads();
   if (warp == 0) {
-    uint64_t places = 0;
-    uint32_t blocks = 0;
+    uint32_t places = 0, blocks = 0;
     for (uint32_t b = lane; b < w.r.batch; b += 32) {
-      places += prefix[b + 1] & 0xffffffffffffull;
-      blocks += (uint32_t)(prefix[b + 1] >> 48);
+      places += prefix[b + 1];
+      blocks += blocks_in[b];
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-      places += __shfl_xor_sync(0xffffffffu, places, o);
-      blocks += __shfl_xor_sync(0xffffffffu, blocks, o);
-    }
+    places = __reduce_add_sync(0xffffffffu, places);
+    blocks = __reduce_add_sync(0xffffffffu, blocks) * G;
     // Whole blocks, taken one by one, end when the last one taken does; equal shares of all places end together, but their blocks have to be joined.
-    const uint64_t ends = (uint64_t)blocks * G <= N ? limits[0] : max((uint64_t)limits[0], places / N + limits[1]);
+    const uint32_t ends = blocks <= N ? limits[0] : max(limits[0], places / N + limits[1]);
     const bool shares = ends > places / N + PT_JOIN;
-    uint64_t sum = 0;
+    uint32_t sum = 0;
     for (uint32_t b0 = 0; b0 < w.r.batch; b0 += 32) {
-      uint64_t v = 0;
-      if (b0 + lane < w.r.batch) v = shares ? prefix[b0 + lane + 1] & 0xffffffffffffull : (prefix[b0 + lane + 1] >> 48) * G;
+      uint32_t v = 0;
+      if (b0 + lane < w.r.batch) v = shares ? prefix[b0 + lane + 1] : blocks_in[b0 + lane] * G;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const uint64_t x = __shfl_up_sync(0xffffffffu, v, o);
+        const uint32_t x = __shfl_up_sync(0xffffffffu, v, o);
         if (lane >= o) v += x;
       }
       if (b0 + lane < w.r.batch) prefix[b0 + lane + 1] = sum + v;
@@ -398,7 +397,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
   }
   __syncthreads();
   const bool shares = limits[0] != 0;
-  const uint64_t total = prefix[w.r.batch], share = shares ? max((total + N - 1) / N, (uint64_t)PT_LIST + 2) : 0;
+  const uint32_t total = prefix[w.r.batch], share = shares ? max((total + N - 1) / N, PT_LIST1 + 2 * PT_TILE1) : 0;
   // The next segment, in shared memory until `done`.  Warps that meet in barriers go on or end together (`together`), whatever became of a wait.
   uint32_t had = 0;
   auto next = [&](bool &ok, auto together) -> uint32_t {  // its address, 0: there is none
@@ -417,7 +416,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
   if (warp == 0) {
     Finder find(w, prefix, seqs, share);
     const uint32_t box = min(w.c.page, PT_KEYS), boxes = PT_KEYS / box;
-    uint32_t it = 0, loads0 = 0, loads1 = 0, tails = 0, handed = 0;
+    uint32_t it = 0, loads0 = 0, loads1 = 0, handed = 0;
     bool ok = true;
     // Blocks are taken from a counter in the workspace as the copies of the one before end; the CTA that draws the last number sets it back.
     auto take = [&]() -> const Segment * {
@@ -439,9 +438,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         more = id < total;
         if (more) find.block(id, g);
       }
-      if (ok) ok = poll(sm + (NE + x) * 8, (handed >> 1 & 1) ^ 1, sm + ABORT, 985);
-      ++handed;
+      if (ok) ok = mbar_wait(sm + (NE + x) * 8, (handed >> 1 & 1) ^ 1, sm + ABORT, 985);
       __syncwarp();
+      ++handed;
       if (lane == 0) {
         segments[x] = g;
         segments[x].more = more;
@@ -490,24 +489,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         ok = __all_sync(0xffffffffu, ok);
       }
     };
-    uint32_t tail_at = 0, tail_from = PT_KEYS;  // the unit with a ragged sequence's last values, and where its zeros begin
-    auto zeros = [&] {
-      if (tail_from < PT_KEYS) {
-        if (ok) ok = mbar_wait(sm + VL * 8, tails & 1, sm + ABORT, 950);
-        __syncwarp();
-        ++tails;
-        if (ok) {
-          const uint32_t n = (PT_KEYS - tail_from) * 8;
-          for (uint32_t i = lane; i < n * SD; i += 32) {
-            *reinterpret_cast<uint4 *>(ring + tail_at * UNIT + i / n * PT_SLAB + tail_from * 128 + i % n * 16) = make_uint4(0, 0, 0, 0);
-          }
-        }
-        fence_proxy_async();
-        __syncwarp();
-        if (leader && ok) mbar_arrive(vz + (tails & 1 ^ 1));
-        tail_from = PT_KEYS;
-      }
-    };
     const Segment *g = take();
     bool first = true;
     while (g) {
@@ -522,42 +503,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         const uint32_t p = t * PT_KEYS + lane * box;
         // no page: rows in front of the pool, which read as zeros
         const int row = (uint32_t)id < w.c.pages ? (int)(((uint32_t)id * G + g->g) * w.c.page + p % w.c.page) : -(int)PT_KEYS;
-        const bool last = t + 1 == t1 && g->ragged;
 #pragma unroll
         for (uint32_t kv = 0; kv < 2; ++kv, ++it) {
           const uint32_t st = it % PT_UNITS;
           wait_asking(sm + (EMPTY + st) * 8, ((it / PT_UNITS) & 1) ^ 1, 900 + st);
           __syncwarp();
-          uint64_t *bar = kv && last ? vl : &full[st];
-          if (leader && ok) mbar_arrive_expect_tx(bar, UNIT);
-          if (leader && ok && kv && last) mbar_arrive(&full[st]);  // its phase goes on without it
+          if (leader && ok) mbar_arrive_expect_tx(&full[st], UNIT);
           __syncwarp();
           if (ok && lane < boxes)
-            for (uint32_t c = 0; c < SD; ++c) tma_load_2d(ring + st * UNIT + c * PT_SLAB + lane * box * 128, kv ? &w.v : &w.k, (int)(c * 64), row, bar);
-        }
-        if (t == t0) zeros();  // of the block before, behind the first copies of this one
-        if (last) {
-          tail_at = (it - 1) % PT_UNITS;
-          tail_from = (uint32_t)max(0, g->s.pos0 + (int)g->s.rows - (int)(t * PT_KEYS));
+            for (uint32_t c = 0; c < SD; ++c) tma_load_2d(ring + st * UNIT + c * PT_SLAB + lane * box * 128, kv ? &w.v : &w.k, (int)(c * 64), row, &full[st]);
         }
       }
-      if (t0 == t1) zeros();
       wait_asking(0, 0, 990);
       first = false;
       g = take();
     }
-    zeros();
     if (leader && *abort_flag) drain_copies(full, it, PT_UNITS);
     if (leader && *abort_flag) drain_copies(qf, loads0, 1);
     if (leader && *abort_flag) drain_copies(qf + 1, loads1, 1);
-    if (leader && *abort_flag) drain_copies(vl, tails, 1);
   } else if (warp == 1) {
     constexpr uint32_t idesc_s = BF16 ? instr_desc_bf16(PT_ROWS, PT_KEYS) : instr_desc_f16(PT_ROWS, PT_KEYS);
     constexpr uint32_t idesc_o = (BF16 ? instr_desc_bf16(PT_ROWS, DH) : instr_desc_f16(PT_ROWS, DH)) | (1u << 16);  // values: keys are the rows of memory (N-major operand)
     const uint32_t q_lo = smem_desc_lo(smem_u32(qs)), k_lo = smem_desc_lo(smem_u32(ring));
     const uint32_t v_lo = ((smem_u32(ring) >> 4) & 0x3FFFu) | ((PT_SLAB >> 4) << 16);  // 64-element groups are a slab apart
     bool ok = true;
-    uint32_t base = 0, tails = 0;  // units before this segment; ragged ends so far
+    uint32_t base = 0;  // units before this segment
     // A half: its tiles in this segment, products with the values made in it, phases of its barriers.  Two of them by name and the code for each: an array that is
     // indexed lies in local memory, whose loads stood between the products.
     struct Half {
@@ -566,7 +536,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     while (next(ok, [](bool x) { return x; })) {
       const uint32_t at = sm + SEGMENTS + (had & 1) * (uint32_t)sizeof(Segment);
       const uint32_t t0 = lds(at + offsetof(Segment, k.t0)), t1 = lds(at + offsetof(Segment, k.t1));
-      const bool ragged = lds(at + offsetof(Segment, ragged));
+      const uint32_t tail = lds(at + offsetof(Segment, tail));
       first.lo = lds(at + offsetof(Segment, k.lo)), first.hi = lds(at + offsetof(Segment, k.hi)), first.made = 0;
       second.lo = lds(at + offsetof(Segment, k.lo) + 4), second.hi = lds(at + offsetof(Segment, k.hi) + 4), second.made = 0;
       for (uint32_t t = t0; t <= t1; ++t) {
@@ -578,8 +548,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
           constexpr uint32_t i = I.value;
           if (vt && t - 1 >= h.lo && t - 1 < h.hi) {
             if (!have_v) {
-              if (ok) ok = ragged && t == t1 ? poll(sm + (VZ + (tails & 1)) * 8, tails >> 1 & 1, sm + ABORT, 921) : poll(sm + (FULL + sv) * 8, (iv / PT_UNITS) & 1, sm + ABORT, 920);
+              if (ok) ok = poll(sm + (FULL + sv) * 8, (iv / PT_UNITS) & 1, sm + ABORT, 920);
               have_v = true;
+              if (tail && t == t1) {  // what the last page holds behind the sequence's end: zeros
+                const uint32_t pieces = tail * 8, from = smem_u32(ring) + sv * UNIT + (PT_KEYS - tail) * 128;
+                for (uint32_t x = lane; x < pieces * SD; x += 32) {
+                  asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(from + x / pieces * PT_SLAB + x % pieces * 16), "r"(0) : "memory");
+                }
+                fence_proxy_async();
+              }
             }
 #pragma unroll
             for (uint32_t part = 0; part < 2; ++part) {
@@ -629,7 +606,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         if (leader && ok && kt) umma_commit(&empty[sk]);
       }
       base += 2 * (t1 - t0);
-      if (ragged) ++tails;
       auto queries_read = [&](auto I, Half &h) {
         constexpr uint32_t i = I.value;
         if (lds(at + offsetof(Segment, k.tokens) + 4 * i)) {
@@ -737,7 +713,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         hide(v, 0);
         hide(u, 1);
         const float tmax = fmaxf(largest(v), largest(u));
-        float sum = probabilities(v, sb + 32);
+        float sum = 0.f;
+        if (!start) sum = probabilities(v, sb + 32);
         if (agree(start || tmax * w.scale2 > m2 + PT_LAZY)) {
           sts(mine, __float_as_uint(tmax));
           meet_other();
@@ -912,7 +889,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 
 template <int SD, bool BF16>
 int launch_tc(cudaStream_t stream, const PagedAttnArgs &w) {
-  const size_t fixed = (size_t)(2 + PT_UNITS) * SD * PT_SLAB + 1024 + PT_SMALL + 8, per = sizeof(uint64_t) + sizeof(PagedSeq);
+  const size_t fixed = (size_t)(2 + PT_UNITS) * SD * PT_SLAB + 1024 + PT_SMALL + 8, per = 8 + sizeof(PagedSeq);
   static bool attr_set[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -942,8 +919,8 @@ int paged_attn_tc(cudaStream_t stream, PagedAttnArgs &w, uint32_t heads) {
     set_error("paged_attn: cuTensorMapEncodeTiled failed with code %d", (int)r);
     return GRETA_ERR_INVALID_ARGS;
   }
-  // Numbers of blocks, and places of a sequence (48 bits) with them, fit their words.
-  GRETA_REQUIRE((uint64_t)(w.r.tokens / (2 * TT) + w.r.batch) * w.c.kv_heads < (1ull << 31) && w.r.tokens / (2 * TT) < 65535, "paged_attn: %u rows of %u heads", w.r.tokens, heads);
+  const uint64_t blocks = w.r.tokens / (2 * TT) + std::min(w.r.batch, w.r.tokens), tiles = (uint64_t)w.c.ld_table * w.c.page / PT_KEYS + 1;
+  GRETA_REQUIRE(blocks * w.c.kv_heads * (tiles * PT_TILE2 + PT_LIST2) < (1ull << 32), "paged_attn: %u rows of %u heads over tables of %u pages", w.r.tokens, heads, w.c.ld_table);
   if (d > 64) return bf16 ? launch_tc<2, true>(stream, w) : launch_tc<2, false>(stream, w);
   return bf16 ? launch_tc<1, true>(stream, w) : launch_tc<1, false>(stream, w);
 }
