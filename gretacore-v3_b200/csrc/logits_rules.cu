@@ -1,9 +1,11 @@
 // Rules on logits (penalties for repeated tokens, biases, a grammar's mask) and the arg-max of what they leave, in one pass.
 //
-// Bytes are what bounds it: logits in and out once, the mask's bits once.  A row belongs to a cluster of CTAs, a slice of the vocabulary to each; a CTA
-// counts the history's ids that fall into its slice in shared memory (integer atomics: the counts do not depend on their order), so there is no table
-// of counts to keep per sequence, to clear or to roll back, and a token that occurs often is adjusted once.  The history is read by every CTA of the
-// row, from L2.
+// Bytes are what bounds it: logits in and out once, the mask's bits once.  A row belongs to a cluster of CTAs, a slice of the vocabulary to each.  A CTA
+// reads the history once and keeps what falls into its slice, then goes through the slice in chunks of 16 tokens a thread: counts of the chunk's ids in shared memory
+// (integer atomics: they do not depend on their order), so there is no table of counts to keep per sequence, to clear or to roll back, and a token that
+// occurs often is adjusted once.  The chunk's logits are asked for before its counts are made.  Clusters of CTAs as large as the rows leave
+// room for.  64 rows of 128256 logits, 4096 ids, 300 biases, masks: 32 us (2.1 TB/s; with one chunk of the whole slice a CTA 59): the phases of a chunk wait for
+// one another, a division and a bias for every token of the text are issued at a few lanes a warp.  One row of 32000, 700 ids: 5.8 us, launch and cluster barriers.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <math.h>
@@ -18,14 +20,15 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t LR_THREADS = 1024, LR_SLICE = 24576;  // tokens whose counts (and biases) a CTA holds at a time: 96 KB each
+constexpr uint32_t LR_EACH = 16;   // tokens of a thread and chunk
+constexpr uint32_t LR_IDS = 2048, LR_BIASES = 512;  // of a slice that are kept; with more of them every chunk reads the caller's again
 constexpr uint32_t LR_SEEN = 0x80000000u;
 
 struct LogitsArgs {
   greta_logits_rules r;
   const void *in;
   void *out;
-  uint32_t ld, ld_out, V, slice;
+  uint32_t ld, ld_out, V;
   int32_t *next;
   uint32_t *pos;
   bool vec, advance;
@@ -66,112 +69,231 @@ __device__ __forceinline__ void warp_first_max(float &best, uint32_t &bi) {
 }
 
 template <int FMT>
-__global__ void __launch_bounds__(LR_THREADS) logits_rules_kernel(const __grid_constant__ LogitsArgs a) {
+__global__ void __launch_bounds__(1024) logits_rules_kernel(const __grid_constant__ LogitsArgs a) {
   typedef typename Elem<FMT>::T T;
-  extern __shared__ uint32_t table[];  // [slice] counts of generated ids, LR_SEEN for any; behind them [slice] 1 + index of the last bias
+  constexpr uint32_t W = 16 / sizeof(T), PACKS = LR_EACH / W;  // tokens of 16 bytes, pieces of a thread and chunk
+  struct alignas(16) Pack { T x[W]; };
+  extern __shared__ uint4 smem4[];
   __shared__ float sv[32];
   __shared__ uint32_t si[32];
+  __shared__ uint32_t kept[2], n_later;  // ids and biases of the slice
   cg::cluster_group cluster = cg::this_cluster();
   pdl_launch_dependents();
   pdl_wait();
   const greta_logits_rules &r = a.r;
-  const uint32_t m = blockIdx.y, rank = blockIdx.x, ctas = gridDim.x, tid = threadIdx.x;
+  const uint32_t m = blockIdx.y, rank = blockIdx.x, ctas = gridDim.x, tid = threadIdx.x, lane = tid & 31, threads = blockDim.x, chunk = threads * LR_EACH;
   const uint32_t per = (((a.V + ctas - 1) / ctas) + 31) & ~31u;  // slices of whole mask words
   const uint32_t lo = min(a.V, rank * per), hi = min(a.V, lo + per);
-  const bool counts = r.ids && (r.repetition || r.frequency || r.presence);
+  const bool counts = r.ids && (r.repetition || r.frequency || r.presence), biased = r.bias_ids;
+  // [chunk] counts of generated ids, LR_SEEN for any; [chunk] 1 + index of the last bias; the slice's ids (LR_SEEN: of the prompt); its biases' tokens and indices
+  uint32_t *table = reinterpret_cast<uint32_t *>(smem4), *biases = table + (counts ? chunk : 0);
+  uint32_t *list = biases + (biased ? chunk : 0), *bias_at = list + (counts ? LR_IDS : 0), *bias_of = bias_at + (biased ? LR_BIASES : 0);
+  uint16_t *later = reinterpret_cast<uint16_t *>(bias_of + (biased ? LR_BIASES : 0));  // [chunk] tokens that ids or biases are about
   const uint32_t n_ids = r.ids ? min(r.n_ids[m], r.ld_ids) : 0;
   const uint32_t n_prompt = r.n_prompt ? r.n_prompt[m] : 0;
   const int32_t *ids = r.ids + (size_t)m * r.ld_ids;
   const float rep = r.ids && r.repetition ? r.repetition[m] : 1.f, freq = r.ids && r.frequency ? r.frequency[m] : 0.f,
               pres = r.ids && r.presence ? r.presence[m] : 0.f;
-  const uint32_t b0 = r.bias_ids ? r.bias_start[m] : 0, b1 = r.bias_ids ? r.bias_start[m + 1] : 0;
+  const uint32_t b0 = biased ? r.bias_start[m] : 0, b1 = biased ? r.bias_start[m + 1] : 0;
   const uint32_t *allowed = r.allowed ? r.allowed + (size_t)m * r.ld_allowed : nullptr;
   const T *in = static_cast<const T *>(a.in) + (size_t)m * a.ld;
   T *out = a.out ? static_cast<T *>(a.out) + (size_t)m * a.ld_out : nullptr;
-  uint32_t *biases = table + a.slice;
-
-  float best = -INFINITY;
-  uint32_t bi = 0xffffffffu;
-  for (uint32_t c0 = lo; c0 < hi; c0 += a.slice) {
-    const uint32_t n = min(a.slice, hi - c0);
-    if (counts || r.bias_ids) {
-      __syncthreads();
-      if (counts)
-        for (uint32_t i = tid; i < n; i += LR_THREADS) table[i] = 0;
-      if (r.bias_ids)
-        for (uint32_t i = tid; i < n; i += LR_THREADS) biases[i] = 0;
-      __syncthreads();
-      if (counts) {
+  // What lies in tokens from .. from + n - 1: count(token - from, of the prompt), bias(token - from, index).
+  auto each_id = [&](uint32_t from, uint32_t n, auto count) {
 #pragma unroll 4
-        for (uint32_t i = tid; i < n_ids; i += LR_THREADS) {
-          const uint32_t t = (uint32_t)ids[i] - c0;
-          if (t < n) {
-            if (i < n_prompt)
-              atomicOr(&table[t], LR_SEEN);
-            else
-              atomicAdd(&table[t], 1u);
-          }
+    for (uint32_t i = tid; i < n_ids; i += threads) {
+      const uint32_t t = (uint32_t)ids[i] - from;
+      if (t < n) count(t, i < n_prompt);
+    }
+  };
+  auto each_bias = [&](uint32_t from, uint32_t n, auto bias) {
+    for (uint32_t i = b0 + tid; i < b1; i += threads) {
+      const uint32_t t = (uint32_t)r.bias_ids[i] - from;
+      if (t < n) bias(t, i - b0 + 1);
+    }
+  };
+  auto to_table = [&](uint32_t t, bool prompt) {
+    if (prompt)
+      atomicOr(&table[t], LR_SEEN);
+    else
+      atomicAdd(&table[t], 1u);
+  };
+  const bool listed = hi - lo > chunk;  // more chunks than one: the lists are read once
+  // Clear to begin with; every entry is cleared again by the one who uses it.
+  for (uint32_t i = tid; i < chunk / 4 * (counts + biased); i += threads) reinterpret_cast<uint4 *>(table)[i] = make_uint4(0, 0, 0, 0);
+  if (tid < 2) kept[tid] = 0;
+  if (tid == 0) n_later = 0;
+  if (listed && (counts || biased)) {
+    __syncthreads();
+    if (counts)
+      for (uint32_t i0 = tid & ~31u; i0 < n_ids; i0 += 4 * threads) {  // places are given out by warps: a thousand single ones take 3 us
+        uint32_t t[4];
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x) {
+          const uint32_t i = i0 + x * threads + lane;
+          t[x] = i < n_ids ? (uint32_t)ids[i] - lo : 0xffffffffu;
+        }
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x) {
+          const uint32_t in_slice = __ballot_sync(0xffffffffu, t[x] < hi - lo);
+          if (!in_slice) continue;
+          uint32_t at = 0;
+          if (lane == 0) at = atomicAdd(&kept[0], __popc(in_slice));
+          at = __shfl_sync(0xffffffffu, at, 0) + __popc(in_slice & ((1u << lane) - 1));
+          if (t[x] < hi - lo && at < LR_IDS) list[at] = t[x] | (i0 + x * threads + lane < n_prompt ? LR_SEEN : 0);
         }
       }
-      for (uint32_t i = b0 + tid; i < b1; i += LR_THREADS) {
-        const uint32_t t = (uint32_t)r.bias_ids[i] - c0;
-        if (t < n) atomicMax(&biases[t], i - b0 + 1);
+    if (biased)
+      each_bias(lo, hi - lo, [&](uint32_t t, uint32_t i) {
+        const uint32_t x = atomicAdd(&kept[1], 1u);
+        if (x < LR_BIASES) {
+          bias_at[x] = t;
+          bias_of[x] = i;
+        }
+      });
+  }
+
+  float best = -INFINITY;
+  uint32_t bi = 0xffffffffu, above = 0;  // above: the largest that the warp has seen, as an ordered integer
+  for (uint32_t c0 = lo; c0 < hi; c0 += chunk) {
+    const uint32_t n = min(chunk, hi - c0), whole = a.vec ? n / W : 0;
+    Pack p[PACKS];
+    uint32_t word[PACKS];
+#pragma unroll
+    for (uint32_t k = 0; k < PACKS; ++k) {
+      const uint32_t i = k * threads + tid;
+      word[k] = 0xffffffffu;
+      if (i < whole) {
+        p[k] = *reinterpret_cast<const Pack *>(in + c0 + i * W);  // c0 is a multiple of 32
+        if (allowed) word[k] = allowed[(c0 + i * W) / 32];
+      }
+    }
+    if (counts || biased) {
+      __syncthreads();  // the tables are clear, the lists are there
+      if (counts) {
+        if (listed && kept[0] <= LR_IDS) {
+          for (uint32_t i = tid; i < kept[0]; i += threads) {
+            const uint32_t t = (list[i] & ~LR_SEEN) + lo - c0;
+            if (t < n) to_table(t, list[i] & LR_SEEN);
+          }
+        } else {
+          each_id(c0, n, to_table);
+        }
+      }
+      if (biased) {
+        if (listed && kept[1] <= LR_BIASES) {
+          for (uint32_t i = tid; i < kept[1]; i += threads) {
+            const uint32_t t = bias_at[i] + lo - c0;
+            if (t < n) atomicMax(&biases[t], bias_of[i]);
+          }
+        } else {
+          each_bias(c0, n, [&](uint32_t t, uint32_t i) { atomicMax(&biases[t], i); });
+        }
       }
       __syncthreads();
     }
     // Every operation rounds once, in the order of the rules: no product is folded into the sum behind it.
-    auto rule = [&](float x, uint32_t t, uint32_t word) {
-      if (counts) {
-        const uint32_t c = table[t - c0];
-        if (c) {
-          x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
-          const uint32_t k = c & ~LR_SEEN;
-          if (k) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)k)), pres);
-        }
+    auto rule = [&](float x, uint32_t t, uint32_t word, uint32_t c, uint32_t b) {
+      if (c) {
+        x = x > 0.f ? __fdiv_rn(x, rep) : __fmul_rn(x, rep);
+        const uint32_t k = c & ~LR_SEEN;
+        if (k) x = __fsub_rn(__fsub_rn(x, __fmul_rn(freq, (float)k)), pres);
       }
-      if (r.bias_ids) {
-        const uint32_t b = biases[t - c0];
-        if (b) x = __fadd_rn(x, r.bias[b0 + b - 1]);
-      }
+      if (b) x = __fadd_rn(x, r.bias[b0 + b - 1]);
       if (!(word >> (t & 31) & 1)) x = -INFINITY;
       return Elem<FMT>::store(x);
     };
     auto look = [&](T y, uint32_t t) {
       float v = Elem<FMT>::load(y);
       if (v != v) v = t ? -INFINITY : INFINITY;  // as greta_cuda_argmax
-      if (v > best || bi == 0xffffffffu) {       // a thread's tokens ascend
+      if (better(v, t, best, bi)) {              // in any order
         best = v;
         bi = t;
       }
     };
-    if (a.vec) {
-      constexpr uint32_t W = 16 / sizeof(T);  // tokens of 16 bytes; c0 is a multiple of 32
-      struct alignas(16) Pack { T x[W]; };
-      const uint32_t whole = n / W;
-#pragma unroll 2
-      for (uint32_t i = tid; i < whole; i += LR_THREADS) {
-        const uint32_t t = c0 + i * W;
-        Pack p = *reinterpret_cast<const Pack *>(in + t);
-        const uint32_t word = allowed ? allowed[t / 32] : 0xffffffffu;
+    auto single = [&](uint32_t t) {
+      uint32_t c = 0, b = 0;
+      if (counts) {
+        c = table[t - c0];
+        if (c) table[t - c0] = 0;
+      }
+      if (biased) {
+        b = biases[t - c0];
+        if (b) biases[t - c0] = 0;
+      }
+      const T y = rule(Elem<FMT>::load(in[t]), t, allowed ? allowed[t / 32] : 0xffffffffu, c, b);
+      if (out) out[t] = y;
+      look(y, t);
+    };
+    // Tokens that neither ids nor biases are about need the mask alone.  The others stay as they are for now and are gathered: a division for a lane or two of every
+    // warp and token cost more than all the rest (64 rows of 128256: 56 us).
+    uint32_t about = 0;      // bits: of the thread's tokens
+    float most = -INFINITY;  // of those that are done with; a NaN is none
 #pragma unroll
-        for (uint32_t e = 0; e < W; ++e) p.x[e] = rule(Elem<FMT>::load(p.x[e]), t + e, word);
-        if (out) *reinterpret_cast<Pack *>(out + t) = p;
+    for (uint32_t k = 0; k < PACKS; ++k) {
+      const uint32_t i = k * threads + tid, t = c0 + i * W;
+      if (i < whole) {
+        uint32_t there[W];
 #pragma unroll
-        for (uint32_t e = 0; e < W; ++e) look(p.x[e], t + e);
+        for (uint32_t e = 0; e < W; e += 4) {
+          const uint4 x = counts ? *reinterpret_cast<const uint4 *>(table + i * W + e) : make_uint4(0, 0, 0, 0);
+          const uint4 y = biased ? *reinterpret_cast<const uint4 *>(biases + i * W + e) : make_uint4(0, 0, 0, 0);
+          there[e] = x.x | y.x, there[e + 1] = x.y | y.y, there[e + 2] = x.z | y.z, there[e + 3] = x.w | y.w;
+        }
+        const uint32_t seen = word[k] >> (t & 31);
+#pragma unroll
+        for (uint32_t e = 0; e < W; ++e) {
+          if (there[e]) {
+            about |= 1u << (k * W + e);
+          } else {
+            if (!(seen >> e & 1)) p[k].x[e] = Elem<FMT>::store(-INFINITY);
+            most = fmaxf(most, Elem<FMT>::load(p[k].x[e]));
+          }
+        }
+        if (out) *reinterpret_cast<Pack *>(out + t) = p[k];
       }
-      const uint32_t t = c0 + whole * W + tid;
-      if (t < c0 + n) {
-        const T y = rule(Elem<FMT>::load(in[t]), t, allowed ? allowed[t / 32] : 0xffffffffu);
-        if (out) out[t] = y;
-        look(y, t);
+    }
+    // Where the largest lies is looked for only when it is above all that the warp has seen.
+    const uint32_t key = __float_as_uint(most) ^ ((uint32_t)((int)__float_as_uint(most) >> 31) | 0x80000000u), highest = __reduce_max_sync(0xffffffffu, key);
+    if (highest > above) {
+      above = highest;
+      if (key == highest) {
+        uint32_t at = 0xffffffffu;
+#pragma unroll
+        for (int x = (int)LR_EACH - 1; x >= 0; --x) {
+          const uint32_t i = (uint32_t)x / W * threads + tid;
+          if (i < whole && !(about >> x & 1) && Elem<FMT>::load(p[x / W].x[x % W]) == most) at = c0 + i * W + (uint32_t)x % W;
+        }
+        if (at != 0xffffffffu && better(most, at, best, bi)) {
+          best = most;
+          bi = at;
+        }
       }
-    } else {
-#pragma unroll 2
-      for (uint32_t t = c0 + tid; t < c0 + n; t += LR_THREADS) {
-        const T y = rule(Elem<FMT>::load(in[t]), t, allowed ? allowed[t / 32] : 0xffffffffu);
-        if (out) out[t] = y;
-        look(y, t);
+    }
+    if (c0 == 0 && tid == 0 && whole && !(about & 1)) look(p[0].x[0], 0);  // NaN counts in the first place
+    if (__any_sync(0xffffffffu, about)) {
+      uint32_t before = __popc(about);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t x = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= (uint32_t)o) before += x;
       }
+      uint32_t at = 0;
+      if (lane == 31) at = atomicAdd(&n_later, before);
+      at = __shfl_sync(0xffffffffu, at, 31) + before - __popc(about);
+      for (; about; about &= about - 1) {
+        const uint32_t x = __ffs(about) - 1;
+        later[at++] = (uint16_t)((x / W * threads + tid) * W + x % W);
+      }
+    }
+    // what is no whole piece, or rows that do not begin at 16-byte boundaries
+    for (uint32_t t = c0 + whole * W + tid; t < c0 + n; t += threads) single(t);
+    if (counts || biased) {
+      __syncthreads();
+      const uint32_t n = n_later;
+      for (uint32_t i = tid; i < n; i += threads) single(c0 + later[i]);
+      __syncthreads();
+      if (tid == 0) n_later = 0;
     }
   }
   if (!a.next) return;
@@ -183,8 +305,8 @@ __global__ void __launch_bounds__(LR_THREADS) logits_rules_kernel(const __grid_c
   }
   __syncthreads();
   if (w == 0) {
-    best = sv[l];
-    bi = si[l];
+    best = l < threads / 32 ? sv[l] : -INFINITY;
+    bi = l < threads / 32 ? si[l] : 0xffffffffu;
     warp_first_max(best, bi);
     __syncwarp();
     if (l == 0) {
@@ -221,18 +343,38 @@ template <int FMT>
 int launch_rules(cudaStream_t stream, LogitsArgs &a, uint32_t M) {
   // As the arg-max: rows that one CTA covers with a few loads per thread stay with it.
   const unsigned ctas = a.V <= 4096 ? 1 : (a.V <= 8192 ? 2 : (a.V <= 16384 ? 4 : 8));
-  const uint32_t per = (((a.V + ctas - 1) / ctas) + 31) & ~31u;
-  a.slice = std::min(LR_SLICE, per);
-  const bool counts = a.r.ids && (a.r.repetition || a.r.frequency || a.r.presence);
-  const size_t smem = counts || a.r.bias_ids ? (size_t)a.slice * 4 * (a.r.bias_ids ? 2 : 1) : 0;
-  static bool attr_set[64] = {};
+  // One chunk per CTA where the rows' clusters run at the same time (a GPC holds two of eight CTAs of 1024 threads, four of 512): latency counts.  Else CTAs of 256
+  // threads, four an SM, whose phases overlap.  Vocabulary 128256, 4096 ids, 300 biases, masks: 14 rows 10.6 us with 1024 threads, 18 rows 17 with 512 and 23 with 256,
+  // 64 rows 35 with 512 and 32 with 256.
+  constexpr uint32_t SIZES[2] = {1024, 512};
+  static int clusters[64][2] = {};  // 1 + clusters of each size that run at a time
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || !attr_set[dev]) {
-    GRETA_CUDA_TRY(cudaFuncSetAttribute(logits_rules_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(LR_SLICE * 8)));
-    if (dev >= 0 && dev < 64) attr_set[dev] = true;
-  }
-  GRETA_CUDA_TRY(launch_pdl_cluster(logits_rules_kernel<FMT>, dim3(ctas, M), dim3(LR_THREADS), ctas, smem, stream, a));
+  if (dev < 0 || dev >= 64) dev = 0;
+  for (int i = 0; i < 2; ++i)
+    if (!clusters[dev][i]) {
+      const uint32_t bytes = (2 * SIZES[i] * LR_EACH + LR_IDS + 2 * LR_BIASES) * 4 + SIZES[i] * LR_EACH * 2;
+      if (i == 0) GRETA_CUDA_TRY(cudaFuncSetAttribute(logits_rules_kernel<FMT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(8);
+      cfg.blockDim = dim3(SIZES[i]);
+      cfg.dynamicSmemBytes = bytes;
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      at[0].val.clusterDim.x = 8;
+      at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      int n = 0;
+      GRETA_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, logits_rules_kernel<FMT>, &cfg));
+      clusters[dev][i] = n + 1;
+    }
+  const uint32_t most = M < (uint32_t)clusters[dev][0] ? SIZES[0] : M < (uint32_t)clusters[dev][1] ? SIZES[1] : 256;
+  const uint32_t needed = (((a.V + ctas - 1) / ctas + LR_EACH - 1) / LR_EACH + 31) & ~31u;  // threads that one chunk takes
+  const uint32_t threads = std::max(128u, std::min(needed, most)), chunk = threads * LR_EACH;
+  const bool counts = a.r.ids && (a.r.repetition || a.r.frequency || a.r.presence);
+  const size_t smem = ((size_t)(counts ? chunk + LR_IDS : 0) + (a.r.bias_ids ? chunk + 2 * LR_BIASES : 0)) * 4 + (counts || a.r.bias_ids ? chunk * 2 : 0);
+  GRETA_CUDA_TRY(launch_pdl_cluster(logits_rules_kernel<FMT>, dim3(ctas, M), dim3(threads), ctas, smem, stream, a));
   return launched("logits_rules_kernel");
 }
 

@@ -18,6 +18,7 @@ using namespace greta;
 namespace {
 
 constexpr uint32_t PA_THREADS = 256;
+constexpr int PA_AHEAD = 3;  // units of a thread that are loaded before anything else: all of a token of 64 + 8 heads of 128
 
 struct AppendArgs {
   greta_paged_cache c;
@@ -28,6 +29,7 @@ struct AppendArgs {
   int q_fmt;
   bool interleaved;
   float amplitude;
+  uint32_t by_units, by_pieces;  // 2^32 over a head's units and pieces, rounded up: division by multiplication
   uint64_t turn[64];  // 2^64 * freq / (2 pi)
 };
 
@@ -36,25 +38,6 @@ __device__ __forceinline__ float load1(const void *p, size_t i) {
   if (FMT == GRETA_FMT_F32) return static_cast<const float *>(p)[i];
   if (FMT == GRETA_FMT_F16) return __half2float(static_cast<const __half *>(p)[i]);
   return __bfloat162float(static_cast<const __nv_bfloat16 *>(p)[i]);
-}
-template <int FMT>
-__device__ __forceinline__ void load8(const void *p, size_t i, float (&x)[8]) {
-  if (FMT == GRETA_FMT_F32) {
-    const float4 a = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i), b = *reinterpret_cast<const float4 *>(static_cast<const float *>(p) + i + 4);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-  } else {
-    const uint4 a = *reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(p) + i);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (FMT == GRETA_FMT_F16) {
-        const float2 f = h2_to_f2(w[e]);
-        x[2 * e] = f.x, x[2 * e + 1] = f.y;
-      } else {
-        x[2 * e] = __uint_as_float(w[e] << 16), x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-      }
-    }
-  }
 }
 __device__ __forceinline__ void store1(void *p, size_t i, int fmt, float x) {
   if (fmt == GRETA_FMT_F32)
@@ -85,13 +68,80 @@ __device__ __forceinline__ void store8(void *p, size_t i, int fmt, const float (
   *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(p) + i) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// VEC: the rotated part is whole groups of eight pairs (and a head whole groups of eight elements, always).
-template <int FMT, bool VEC>
+// Sixteen values as they lie in memory.
+template <int FMT>
+struct Raw {
+  uint4 w[FMT == GRETA_FMT_F32 ? 4 : 2];
+  static constexpr int HALF = FMT == GRETA_FMT_F32 ? 2 : 1;
+  __device__ __forceinline__ void load(const void *p, size_t i, int half) {  // eight of them
+    const uint4 *src = reinterpret_cast<const uint4 *>(FMT == GRETA_FMT_F32 ? static_cast<const void *>(static_cast<const float *>(p) + i)
+                                                                              : static_cast<const void *>(static_cast<const uint16_t *>(p) + i));
+#pragma unroll
+    for (int j = 0; j < HALF; ++j) w[half * HALF + j] = src[j];
+  }
+  __device__ __forceinline__ void values(int half, float (&x)[8]) const {
+#pragma unroll
+    for (int j = 0; j < HALF; ++j) {
+      const uint4 v = w[half * HALF + j];
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (FMT == GRETA_FMT_F32) {
+          x[4 * j + e] = __uint_as_float(u[e]);
+        } else if (FMT == GRETA_FMT_F16) {
+          const float2 f = h2_to_f2(u[e]);
+          x[2 * e] = f.x, x[2 * e + 1] = f.y;
+        } else {
+          x[2 * e] = __uint_as_float(u[e] << 16), x[2 * e + 1] = __uint_as_float(u[e] & 0xffff0000u);
+        }
+      }
+    }
+  }
+};
+
+// What a thread moves at a time: eight pairs, or (`straight`) eight elements that are not rotated, of a head of q, k or v.
+struct Unit {
+  uint32_t h, e0, e1;  // head (of q, then of k, then of v); elements
+  bool straight;
+};
+
+template <int FMT>
 __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_constant__ AppendArgs a) {
   __shared__ float cs[64], sn[64];
   pdl_launch_dependents();
   pdl_wait();
-  const uint32_t tok = blockIdx.x, tid = threadIdx.x;
+  const uint32_t tok = blockIdx.x, tid = threadIdx.x, d = a.c.dim, half = a.dims / 2, G = a.c.kv_heads, hq = a.q ? a.heads : 0;
+  const uint32_t first = blockIdx.y * PA_THREADS + tid, step = gridDim.y * PA_THREADS, turned = a.dims / 16, straight = (d - a.dims) / 8, units = turned + straight, pieces = d / 8;
+  const uint32_t of_qk = (hq + G) * units, all = of_qk + G * pieces;
+  auto unit = [&](uint32_t i) {
+    Unit u;
+    if (i < of_qk) {
+      u.h = __umulhi(i, a.by_units);
+      const uint32_t x = i - u.h * units;
+      u.straight = x >= turned;
+      u.e0 = u.straight ? a.dims + 8 * (x - turned) : a.interleaved ? 16 * x : 8 * x;
+      u.e1 = a.interleaved ? 16 * x + 8 : half + 8 * x;
+    } else {
+      const uint32_t v = __umulhi(i - of_qk, a.by_pieces);
+      u.h = hq + G + v;
+      u.straight = true;
+      u.e0 = 8 * (i - of_qk - v * pieces);
+      u.e1 = 0;
+    }
+    return u;
+  };
+  auto load = [&](const Unit &u, Raw<FMT> &r) {
+    const void *src = u.h < hq ? a.q : u.h < hq + G ? a.k : a.v;
+    const size_t at = u.h < hq ? (size_t)tok * a.ld_q + (size_t)u.h * d : u.h < hq + G ? (size_t)tok * a.ld_k + (size_t)(u.h - hq) * d : (size_t)tok * a.ld_v + (size_t)(u.h - hq - G) * d;
+    r.load(src, at + u.e0, 0);
+    if (!u.straight) r.load(src, at + u.e1, 1);
+  };
+  // The first units are on their way while the token's sequence is looked for: neither depends on the other.  (A token behind the last sequence reads its
+  // rows of the buffers for nothing.)
+  Raw<FMT> raw[PA_AHEAD];
+#pragma unroll
+  for (int x = 0; x < PA_AHEAD; ++x)
+    if (first + x * step < all) load(unit(first + x * step), raw[x]);
   // The token's sequence: the last whose start is at or before it (starts do not decrease; empty ones in between are passed over).
   uint32_t before = 0;
   for (uint32_t b0 = 0;; b0 += PA_THREADS) {
@@ -106,7 +156,6 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
   if (tok - s.first >= s.rows || pos < 0) return;
   const int page = __ldcg(a.c.table + (size_t)b * a.c.ld_table + (uint32_t)pos / a.c.page);
   const bool held = page >= 0 && (uint32_t)page < a.c.pages;
-  const uint32_t d = a.c.dim, half = a.dims / 2, G = a.c.kv_heads;
   if (tid < half) {
     const uint64_t t = (uint64_t)(uint32_t)pos * a.turn[tid];
     float sine, cosine;
@@ -115,65 +164,96 @@ __global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_c
     sn[tid] = sine * a.amplitude;
   }
   __syncthreads();
-  const size_t row = ((size_t)(held ? page : 0) * G * a.c.page + (uint32_t)pos % a.c.page) * d, step = (size_t)a.c.page * d;  // of kv head 0; to the next head
-  const uint32_t hq = a.q ? a.heads : 0, at = blockIdx.y * PA_THREADS + tid, all = gridDim.y * PA_THREADS;
-  // Heads' units: eight pairs (or one), then eight elements (or one) of the part that is not rotated; all heads of q, then of k.
-  const uint32_t turned = VEC ? a.dims / 16 : half, straight = (d - a.dims) / (VEC ? 8 : 1), units = turned + straight;
-  for (uint32_t i = at; i < (hq + G) * units; i += all) {
-    const uint32_t h = i / units, u = i % units;
-    const bool is_q = h < hq;
-    const void *src = is_q ? a.q : a.k;
-    const size_t from = is_q ? (size_t)tok * a.ld_q + (size_t)h * d : (size_t)tok * a.ld_k + (size_t)(h - hq) * d;
-    void *dst = is_q ? a.q_out : a.c.k;
-    const size_t to = is_q ? (size_t)tok * a.ld_q_out + (size_t)h * d : row + (h - hq) * step;
+  const size_t row = ((size_t)(held ? page : 0) * G * a.c.page + (uint32_t)pos % a.c.page) * d, next_head = (size_t)a.c.page * d;  // of KV head 0
+  auto store = [&](const Unit &u, const Raw<FMT> &r) {
+    const bool is_q = u.h < hq;
+    if (!is_q && !held) return;
+    void *dst = is_q ? a.q_out : u.h < hq + G ? a.c.k : a.c.v;
+    const size_t to = is_q ? (size_t)tok * a.ld_q_out + (size_t)u.h * d : row + (u.h < hq + G ? u.h - hq : u.h - hq - G) * next_head;
     const int fmt = is_q ? a.q_fmt : a.c.fmt;
-    if (!is_q && !held) continue;
-    if (u < turned) {
-      const bool near = a.interleaved;
-      if (VEC) {
-        const uint32_t e0 = near ? 16 * u : 8 * u, e1 = near ? 16 * u + 8 : half + 8 * u;
-        float x[8], y[8];
-        load8<FMT>(src, from + e0, x);
-        load8<FMT>(src, from + e1, y);
-        if (near) {
+    float x[8], y[8];
+    r.values(0, x);
+    if (!u.straight) {
+      r.values(1, y);
+      const uint32_t p = (a.interleaved ? u.e0 / 16 : u.e0 / 8) * 8;  // its pairs
+      if (a.interleaved) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float c0 = cs[8 * u + e], s0 = sn[8 * u + e], c1 = cs[8 * u + 4 + e], s1 = sn[8 * u + 4 + e];
-            const float x0 = x[2 * e], x1 = x[2 * e + 1], y0 = y[2 * e], y1 = y[2 * e + 1];
-            x[2 * e] = x0 * c0 - x1 * s0, x[2 * e + 1] = x1 * c0 + x0 * s0;
-            y[2 * e] = y0 * c1 - y1 * s1, y[2 * e + 1] = y1 * c1 + y0 * s1;
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float c = cs[8 * u + e], z = sn[8 * u + e], x0 = x[e], y0 = y[e];
-            x[e] = x0 * c - y0 * z, y[e] = y0 * c + x0 * z;
-          }
+        for (int e = 0; e < 4; ++e) {
+          const float c0 = cs[p + e], s0 = sn[p + e], c1 = cs[p + 4 + e], s1 = sn[p + 4 + e];
+          const float x0 = x[2 * e], x1 = x[2 * e + 1], y0 = y[2 * e], y1 = y[2 * e + 1];
+          x[2 * e] = x0 * c0 - x1 * s0, x[2 * e + 1] = x1 * c0 + x0 * s0;
+          y[2 * e] = y0 * c1 - y1 * s1, y[2 * e + 1] = y1 * c1 + y0 * s1;
         }
-        store8(dst, to + e0, fmt, x);
-        store8(dst, to + e1, fmt, y);
       } else {
-        const uint32_t e0 = near ? 2 * u : u, e1 = near ? 2 * u + 1 : half + u;
-        const float x = load1<FMT>(src, from + e0), y = load1<FMT>(src, from + e1), c = cs[u], z = sn[u];
-        store1(dst, to + e0, fmt, x * c - y * z);
-        store1(dst, to + e1, fmt, y * c + x * z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float c = cs[p + e], z = sn[p + e], x0 = x[e], y0 = y[e];
+          x[e] = x0 * c - y0 * z, y[e] = y0 * c + x0 * z;
+        }
       }
-    } else if (VEC) {
-      const uint32_t e = a.dims + 8 * (u - turned);
-      float x[8];
-      load8<FMT>(src, from + e, x);
-      store8(dst, to + e, fmt, x);
+      store8(dst, to + u.e1, fmt, y);
+    }
+    store8(dst, to + u.e0, fmt, x);
+  };
+#pragma unroll
+  for (int x = 0; x < PA_AHEAD; ++x)
+    if (first + x * step < all) store(unit(first + x * step), raw[x]);
+  for (uint32_t i = first + PA_AHEAD * step; i < all; i += step) {
+    const Unit u = unit(i);
+    load(u, raw[0]);
+    store(u, raw[0]);
+  }
+}
+
+// The same where the rotated part is no whole groups of eight pairs: a pair or an element at a time.
+template <int FMT>
+__global__ void __launch_bounds__(PA_THREADS) paged_append_pairs_kernel(const __grid_constant__ AppendArgs a) {
+  __shared__ float cs[64], sn[64];
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t tok = blockIdx.x, tid = threadIdx.x;
+  uint32_t before = 0;
+  for (uint32_t b0 = 0;; b0 += PA_THREADS) {
+    const uint32_t n = __syncthreads_count(b0 + tid < a.r.batch && __ldcg(a.r.start + b0 + tid) <= tok);
+    before += n;
+    if (n < PA_THREADS) break;
+  }
+  if (before == 0) return;
+  const uint32_t b = before - 1;
+  const PagedSeq s = paged_seq(a.r, a.c.ld_table * a.c.page, b);
+  const int pos = s.pos0 + (int)(tok - s.first);
+  if (tok - s.first >= s.rows || pos < 0) return;
+  const int page = __ldcg(a.c.table + (size_t)b * a.c.ld_table + (uint32_t)pos / a.c.page);
+  const bool held = page >= 0 && (uint32_t)page < a.c.pages;
+  const uint32_t d = a.c.dim, half = a.dims / 2, G = a.c.kv_heads, hq = a.q ? a.heads : 0;
+  if (tid < half) {
+    const uint64_t t = (uint64_t)(uint32_t)pos * a.turn[tid];
+    float sine, cosine;
+    sincospif((float)(int32_t)(t >> 32) * 4.656612873077393e-10f, &sine, &cosine);
+    cs[tid] = cosine * a.amplitude;
+    sn[tid] = sine * a.amplitude;
+  }
+  __syncthreads();
+  const size_t row = ((size_t)(held ? page : 0) * G * a.c.page + (uint32_t)pos % a.c.page) * d, next_head = (size_t)a.c.page * d;
+  const uint32_t units = half + d - a.dims;
+  for (uint32_t i = blockIdx.y * PA_THREADS + tid; i < (hq + 2 * G) * units; i += gridDim.y * PA_THREADS) {
+    const uint32_t h = i / units, u = i % units;
+    const bool is_q = h < hq, is_v = h >= hq + G;
+    if (!is_q && !held) continue;
+    const void *src = is_q ? a.q : is_v ? a.v : a.k;
+    const size_t from = is_q ? (size_t)tok * a.ld_q + (size_t)h * d : is_v ? (size_t)tok * a.ld_v + (size_t)(h - hq - G) * d : (size_t)tok * a.ld_k + (size_t)(h - hq) * d;
+    void *dst = is_q ? a.q_out : is_v ? a.c.v : a.c.k;
+    const size_t to = is_q ? (size_t)tok * a.ld_q_out + (size_t)h * d : row + (is_v ? h - hq - G : h - hq) * next_head;
+    const int fmt = is_q ? a.q_fmt : a.c.fmt;
+    if (u < half) {
+      const uint32_t e0 = a.interleaved ? 2 * u : u, e1 = a.interleaved ? 2 * u + 1 : half + u;
+      const float x = load1<FMT>(src, from + e0), y = load1<FMT>(src, from + e1), c = is_v ? 1.f : cs[u], z = is_v ? 0.f : sn[u];
+      store1(dst, to + e0, fmt, is_v ? x : x * c - y * z);
+      store1(dst, to + e1, fmt, is_v ? y : y * c + x * z);
     } else {
-      const uint32_t e = a.dims + (u - turned);
+      const uint32_t e = a.dims + (u - half);
       store1(dst, to + e, fmt, load1<FMT>(src, from + e));
     }
-  }
-  if (!held) return;
-  for (uint32_t i = at; i < G * (d / 8); i += all) {
-    const uint32_t h = i / (d / 8), e = i % (d / 8) * 8;
-    float x[8];
-    load8<FMT>(a.v, (size_t)tok * a.ld_v + (size_t)h * d + e, x);
-    store8(a.c.v, row + h * step + e, a.c.fmt, x);
   }
 }
 
@@ -218,14 +298,18 @@ extern "C" int greta_cuda_paged_append(greta_stream_t stream, const greta_paged_
   if (rows->tokens == 0) return GRETA_OK;
   // Few tokens: heads spread over more CTAs, down to a unit or two per thread.
   const bool vec = a.dims % 16 == 0;
-  const uint32_t units = ((q ? heads : 0) + G) * (vec ? a.dims / 16 + (d - a.dims) / 8 : a.dims / 2 + d - a.dims);
+  const uint32_t units = vec ? ((q ? heads : 0) + G) * (a.dims / 16 + (d - a.dims) / 8) + G * d / 8 : ((q ? heads : 0) + 2 * G) * (d - a.dims / 2);
+  if (vec) {
+    a.by_units = (uint32_t)((0x100000000ull + a.dims / 16 + (d - a.dims) / 8 - 1) / (a.dims / 16 + (d - a.dims) / 8));
+    a.by_pieces = (uint32_t)((0x100000000ull + d / 8 - 1) / (d / 8));
+  }
   const uint32_t parts = rows->tokens >= 1024 ? 1 : std::max(1u, std::min({(units + PA_THREADS - 1) / PA_THREADS, 1024 / rows->tokens, 64u}));
   auto go = [&](auto kernel) { return launch_pdl(kernel, dim3(rows->tokens, parts), dim3(PA_THREADS), 0, static_cast<cudaStream_t>(stream), a); };
   if (fmt == GRETA_FMT_F32)
-    GRETA_CUDA_TRY(vec ? go(paged_append_kernel<GRETA_FMT_F32, true>) : go(paged_append_kernel<GRETA_FMT_F32, false>));
+    GRETA_CUDA_TRY(vec ? go(paged_append_kernel<GRETA_FMT_F32>) : go(paged_append_pairs_kernel<GRETA_FMT_F32>));
   else if (fmt == GRETA_FMT_F16)
-    GRETA_CUDA_TRY(vec ? go(paged_append_kernel<GRETA_FMT_F16, true>) : go(paged_append_kernel<GRETA_FMT_F16, false>));
+    GRETA_CUDA_TRY(vec ? go(paged_append_kernel<GRETA_FMT_F16>) : go(paged_append_pairs_kernel<GRETA_FMT_F16>));
   else
-    GRETA_CUDA_TRY(vec ? go(paged_append_kernel<GRETA_FMT_BF16, true>) : go(paged_append_kernel<GRETA_FMT_BF16, false>));
+    GRETA_CUDA_TRY(vec ? go(paged_append_kernel<GRETA_FMT_BF16>) : go(paged_append_pairs_kernel<GRETA_FMT_BF16>));
   return launched("paged_append_kernel");
 }

@@ -106,6 +106,13 @@ def test_rules(g, t, kw):
     check(g, Case(t=t, seed=kw["V"], **kw))
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("kw", [dict(hist=300, biases=100, mask=True), dict(hist=30000, biases=20000, mask=True), dict(hist=20000), dict(biases=20000), dict(mask=True)])
+def test_rules_of_many_rows(g, t, kw):
+    """Several chunks a CTA: ids and biases of a slice kept, and more of them than are kept."""
+    check(g, Case(M=20, V=50257, t=t, seed=9, **kw))
+
+
 @pytest.mark.parametrize("pen", [(), ("repetition",), ("frequency",), ("presence", "frequency")])
 @pytest.mark.parametrize("prompt", [True, False])
 def test_single_rules(g, pen, prompt):
