@@ -1,8 +1,8 @@
 // New rows of a ragged batch into a paged cache: queries and keys rotated to their positions on the way, keys and values to their pages.
 //
 // Bytes are what bounds it: q, k and v in, q and the two cache rows out, nothing else.  A CTA takes a token (or a part of its heads where there are few
-// tokens): it finds the token's sequence by counting starts, takes the cosines and sines of all pairs once for all heads, then moves
-// eight pairs a thread (two 16-byte loads of 16-bit values, four of 32-bit).
+// tokens): it finds the token's sequence by counting starts, takes the cosines and sines of all pairs once for all heads, then turns
+// eight pairs a thread (two 16-byte loads of 16-bit values, four of 32-bit), which were asked for before all that.
 //
 // The angle of pair i at position p is p * freq_i.  In fp32 it loses a bit for every doubling of p.  Here freq_i / 2 pi is a 64-bit binary fraction of a turn,
 // made on the host in extended precision: p times it, modulo 2^64, is the fraction of a turn to p * 2^-65, whole turns fall away for nothing, and its
@@ -18,7 +18,10 @@ using namespace greta;
 namespace {
 
 constexpr uint32_t PA_THREADS = 256;
-constexpr int PA_AHEAD = 3;  // units of a thread that are loaded before anything else: all of a token of 64 + 8 heads of 128
+// Units of a thread that are loaded before anything else, and CTAs a SM that the registers leave room for.  16 bits: three, all of a token of 64 + 8 heads of 128 (16384
+// of them: 126 us, 5.3 TB/s; one: 144).  32 bits: one, and more CTAs (8192 tokens of 32 + 32 heads: 98 us, 6.1 TB/s; three: 112).
+__host__ __device__ constexpr int pa_ahead(int fmt) { return fmt == GRETA_FMT_F32 ? 1 : 3; }
+__host__ __device__ constexpr int pa_ctas(int fmt) { return fmt == GRETA_FMT_F32 ? 6 : 3; }
 
 struct AppendArgs {
   greta_paged_cache c;
@@ -106,7 +109,8 @@ struct Unit {
 };
 
 template <int FMT>
-__global__ void __launch_bounds__(PA_THREADS) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(PA_THREADS, pa_ctas(FMT)) paged_append_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int PA_AHEAD = pa_ahead(FMT);
   __shared__ float cs[64], sn[64];
   pdl_launch_dependents();
   pdl_wait();
