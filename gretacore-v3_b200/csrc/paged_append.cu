@@ -18,10 +18,11 @@ using namespace greta;
 namespace {
 
 constexpr uint32_t PA_THREADS = 256;
-// Units of a thread that are loaded before anything else, and CTAs a SM that the registers leave room for.  16 bits: three, all of a token of 64 + 8 heads of 128 (16384
-// of them: 126 us, 5.3 TB/s; one: 144).  32 bits: one, and more CTAs (8192 tokens of 32 + 32 heads: 98 us, 6.1 TB/s; three: 112).
+// Units of a thread that are loaded before anything else, and CTAs a SM that the registers leave room for.  16 bits: three, all of a token of 64 + 8 heads of 128, and
+// four CTAs (16384 of them: 128 us, 5.3 TB/s; three CTAs: 148, five: 154; two units and five CTAs: 133).  32 bits: one, and more CTAs (8192 tokens of 32 + 32 heads: 98 us,
+// 6.1 TB/s; three: 112).
 __host__ __device__ constexpr int pa_ahead(int fmt) { return fmt == GRETA_FMT_F32 ? 1 : 3; }
-__host__ __device__ constexpr int pa_ctas(int fmt) { return fmt == GRETA_FMT_F32 ? 6 : 3; }
+__host__ __device__ constexpr int pa_ctas(int fmt) { return fmt == GRETA_FMT_F32 ? 6 : 4; }
 
 struct AppendArgs {
   greta_paged_cache c;

@@ -29,6 +29,7 @@ constexpr uint32_t PAGED_COUNTER = PAGED_TICKETS / 4 - 1;        // the word tha
 constexpr uint32_t PAGED_MMA_PART = 64 * (128 + 2), PAGED_PART = 256 * (128 + 2);  // floats of a part of a row block
 constexpr size_t PAGED_PARTS = 2 * (size_t)(PAGED_MAX_CTAS * PAGED_MMA_PART > PAGED_TC_CTAS * PAGED_PART ? PAGED_MAX_CTAS * PAGED_MMA_PART : PAGED_TC_CTAS * PAGED_PART);
 
+bool paged_tc_fits(const PagedAttnArgs &w);
 int paged_attn_tc(cudaStream_t stream, PagedAttnArgs &w, uint32_t heads);  // paged_attention_tc.cu
 
 #ifdef __CUDACC__

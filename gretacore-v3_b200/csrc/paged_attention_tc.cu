@@ -906,7 +906,13 @@ int launch_tc(cudaStream_t stream, const PagedAttnArgs &w) {
 
 namespace greta {
 
-// Queries of the cache's type, groups of up to 128; w.k and w.v with boxes of min(page, 128) rows.
+// Places are numbered with 32 bits, of whatever lengths the tables have room for: about a second's work.
+bool paged_tc_fits(const PagedAttnArgs &w) {
+  if (w.group > PT_ROWS) return false;
+  const uint64_t blocks = w.r.tokens / (2 * (PT_ROWS / w.group)) + std::min(w.r.batch, w.r.tokens), tiles = (uint64_t)w.c.ld_table * w.c.page / PT_KEYS + 1;
+  return blocks * w.c.kv_heads < (1ull << 31) / (tiles * PT_TILE2 + PT_LIST2);
+}
+// Queries of the cache's type, where paged_tc_fits; w.k and w.v with boxes of min(page, 128) rows.
 int paged_attn_tc(cudaStream_t stream, PagedAttnArgs &w, uint32_t heads) {
   EncodeTiledFn enc = encode_tiled();
   const uint32_t d = w.c.dim, TT = PT_ROWS / w.group;
@@ -919,8 +925,6 @@ int paged_attn_tc(cudaStream_t stream, PagedAttnArgs &w, uint32_t heads) {
     set_error("paged_attn: cuTensorMapEncodeTiled failed with code %d", (int)r);
     return GRETA_ERR_INVALID_ARGS;
   }
-  const uint64_t blocks = w.r.tokens / (2 * TT) + std::min(w.r.batch, w.r.tokens), tiles = (uint64_t)w.c.ld_table * w.c.page / PT_KEYS + 1;
-  GRETA_REQUIRE(blocks * w.c.kv_heads * (tiles * PT_TILE2 + PT_LIST2) < (1ull << 32), "paged_attn: %u rows of %u heads over tables of %u pages", w.r.tokens, heads, w.c.ld_table);
   if (d > 64) return bf16 ? launch_tc<2, true>(stream, w) : launch_tc<2, false>(stream, w);
   return bf16 ? launch_tc<1, true>(stream, w) : launch_tc<1, false>(stream, w);
 }
