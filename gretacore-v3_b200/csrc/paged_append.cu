@@ -33,7 +33,7 @@ struct AppendArgs {
   int q_fmt;
   bool interleaved;
   float amplitude;
-  uint32_t by_units, by_pieces;  // 2^32 over a head's units and pieces, rounded up: division by multiplication
+  uint32_t by_units, by_pieces;  // 2^31 over a head's units and pieces, rounded up: division by multiplication (exact below 2^31 / 16)
   uint64_t turn[64];  // 2^64 * freq / (2 pi)
 };
 
@@ -121,13 +121,13 @@ __global__ void __launch_bounds__(PA_THREADS, pa_ctas(FMT)) paged_append_kernel(
   auto unit = [&](uint32_t i) {
     Unit u;
     if (i < of_qk) {
-      u.h = __umulhi(i, a.by_units);
+      u.h = __umulhi(2 * i, a.by_units);
       const uint32_t x = i - u.h * units;
       u.straight = x >= turned;
       u.e0 = u.straight ? a.dims + 8 * (x - turned) : a.interleaved ? 16 * x : 8 * x;
       u.e1 = a.interleaved ? 16 * x + 8 : half + 8 * x;
     } else {
-      const uint32_t v = __umulhi(i - of_qk, a.by_pieces);
+      const uint32_t v = __umulhi(2 * (i - of_qk), a.by_pieces);
       u.h = hq + G + v;
       u.straight = true;
       u.e0 = 8 * (i - of_qk - v * pieces);
@@ -305,8 +305,9 @@ extern "C" int greta_cuda_paged_append(greta_stream_t stream, const greta_paged_
   const bool vec = a.dims % 16 == 0;
   const uint32_t units = vec ? ((q ? heads : 0) + G) * (a.dims / 16 + (d - a.dims) / 8) + G * d / 8 : ((q ? heads : 0) + 2 * G) * (d - a.dims / 2);
   if (vec) {
-    a.by_units = (uint32_t)((0x100000000ull + a.dims / 16 + (d - a.dims) / 8 - 1) / (a.dims / 16 + (d - a.dims) / 8));
-    a.by_pieces = (uint32_t)((0x100000000ull + d / 8 - 1) / (d / 8));
+    auto by = [](uint32_t n) { return (0x80000000u + n - 1) / n; };
+    a.by_units = by(a.dims / 16 + (d - a.dims) / 8);
+    a.by_pieces = by(d / 8);
   }
   const uint32_t parts = rows->tokens >= 1024 ? 1 : std::max(1u, std::min({(units + PA_THREADS - 1) / PA_THREADS, 1024 / rows->tokens, 64u}));
   auto go = [&](auto kernel) { return launch_pdl(kernel, dim3(rows->tokens, parts), dim3(PA_THREADS), 0, static_cast<cudaStream_t>(stream), a); };

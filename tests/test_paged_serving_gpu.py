@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 
 import _paged as P
+import test_paged_gpu as T
 from _support import load_package
 
 pytestmark = pytest.mark.gpu
@@ -177,3 +178,16 @@ def test_prompts_said_to_be_longer_than_the_text(g):
         want = P.rules64(x[m], V, ids=ids[m], n_ids=int(n[m]), n_prompt=int(n[m]), repetition=np.float32(1.5), frequency=2.0)
         assert (np.abs(got[m] - want) <= 2.0 ** -23 * np.abs(want)).all()
         assert nxt.download(np.int32)[m] == got[m].argmax()
+
+
+@pytest.mark.parametrize("t,cache", [("f32", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("d,dims,interleaved", [(8, 0, False), (16, 16, False), (16, 16, True), (16, 0, False), (24, 16, False), (32, 32, False)])
+def test_append_of_small_heads(g, t, cache, d, dims, interleaved):
+    """Heads of one unit and of a few."""
+    T.check_append(g, [(3, 20), (1, 9), (40, 40)], 6, 3, d, 8, cache, t, t, dims, interleaved=interleaved)
+
+
+@pytest.mark.parametrize("qt,most", [("f32", 2), ("f16", 2), ("f16", 40)])
+def test_attention_of_many_sequences(g, qt, most):
+    """As many sequences as a call takes, empty ones among them."""
+    P.check_attention([(b % (most + 1), b % (most + 1) + b % 37) for b in range(1024)], 4, 2, 64, 16, "f16", qt, seed=36)
