@@ -9,6 +9,14 @@
 //   tensor memory: scores of tile A and B at columns 0 and 128, each half of which is overwritten by its probabilities (32 columns), outputs at 256 and 384.
 // A row's sums are rescaled only when its maximum has grown by more than 2^8 (probabilities up to 2^8 fit every type); the scores' barrier of a key tile says that
 // the products of the one before are in, so the rows' own threads do that.
+// Probabilities are rounded to the cache's type for the second product (half a step: 2^-11 or 2^-8 of each); the sum of them is taken in fp32 before that.
+//
+// What bounds it: the tensor core (58 % of the time) and the exponentials (special-function unit 59 %, 16 cycles a warp in any type) take turns that do not overlap whole; every
+// row's 64 scores, bounds and sums take the 96 registers that 18 warps leave a thread (a spill in this loop goes to the second-level cache, since tiles leave the first 28 KB:
+// 58 us became 68).  512 rows behind 15872 keys, 64 heads over 8 of 128: 226 us alone (1200 TFLOP/s), 271 when the power limit has lowered the clocks; a prompt of
+// 2048, 32 heads: 45 us; of 8192: 485 (1130 TFLOP/s).
+// Blocks: where there are many, whole ones are drawn from a counter, the longest first (no joining); where drawn ones would leave SMs idle longer than joining takes, all
+// CTAs get equal shares of the places, and the last of a block's CTAs to finish joins its parts in their order.
 #include <math.h>
 #include <stddef.h>
 
@@ -376,6 +384,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
     places = __reduce_add_sync(0xffffffffu, places);
     blocks = __reduce_add_sync(0xffffffffu, blocks) * G;
     // Whole blocks, taken one by one, end when the last one taken does; equal shares of all places end together, but their blocks have to be joined.
+    // Prompt of 2048, 32 heads: 45 us by blocks, 60 by shares; eight drafts of five tokens: 25 and 20.5; three portions and 21 single tokens: 248 and 235.
     const uint32_t ends = blocks <= N ? limits[0] : max(limits[0], places / N + limits[1]);
     const bool shares = ends > places / N + PT_JOIN;
     uint32_t sum = 0;

@@ -476,7 +476,8 @@ GRETA_API int greta_cuda_paged_append(greta_stream_t stream, const greta_paged_c
  * rounded to it, the rest is fp32).  heads: a multiple of kv_heads; scale: above 0.  The new rows' keys and values are in the cache already (greta_cuda_paged_append).  What
  * lies behind a row's position, or in front of its window, does not reach it whatever it is.  Rows without keys are zeros.  o and q do not overlap.
  * workspace: greta_cuda_paged_attn_workspace_bytes(dim) bytes, 16-byte aligned, its first 64 KB zero before the first call; one serves every
- * shape, one call at a time.  Waits in the kernels are bounded; one that gave up shows in greta_cuda_gemm_segments_status.
+ * shape, one call at a time.  Waits in the kernels are bounded; one that gave up shows in greta_cuda_gemm_segments_status, and the workspace is cleared again before the
+ * next call.
  * The ragged form of greta_cuda_attn_decode_batch and greta_cuda_attn_prefill. */
 GRETA_API size_t greta_cuda_paged_attn_workspace_bytes(uint32_t dim);
 GRETA_API int greta_cuda_paged_attn(greta_stream_t stream, const greta_paged_cache *cache, const greta_ragged *rows, const void *q, int q_fmt, uint32_t ld_q,
