@@ -1,5 +1,8 @@
 """Append, attention and rules on logits as a serving loop runs them, and calls at the borders of their forms."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -191,3 +194,10 @@ def test_append_of_small_heads(g, t, cache, d, dims, interleaved):
 def test_attention_of_many_sequences(g, qt, most):
     """As many sequences as a call takes, empty ones among them."""
     P.check_attention([(b % (most + 1), b % (most + 1) + b % 37) for b in range(1024)], 4, 2, 64, 16, "f16", qt, seed=36)
+
+
+def test_first_calls_of_a_process_are_captured(g):
+    """Attributes, occupancies and the error word are asked for while a stream is being captured."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    r = subprocess.run([sys.executable, os.path.join(here, "_fresh_capture.py")], cwd=here, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip().endswith("same"), r.stdout + r.stderr
