@@ -325,8 +325,10 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
           }
         __syncwarp();
         if (lane == 0) mbar_arrive(qread);
-      } else if (MT > 1) {
-        bar_math();  // the rows before have been read
+      } else {
+        bar_math();  // the rows before have been read, and their sums: a segment of no tile writes its own with no other barrier in front
+      }
+      if (MT > 1) {
         for (uint32_t r = warp; r < ROWS; r += PM_WARPS) {
           float2 x[DH / 64];
           float most = 0.f;

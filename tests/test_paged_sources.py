@@ -1,0 +1,17 @@
+"""Rules of the paged operators' sources that no run shows reliably."""
+import os
+
+from test_kernel_sources import CSRC, _blocks, _code
+
+
+def test_sums_of_a_row_block_are_read_before_the_next_are_written():
+    """The math warps of the few-row attention write sums of weights, meet, and read all warps' sums; a block that falls to one CTA meets no more behind that.  So the next segment has
+    a barrier in front of its own sums whether it has tiles (the tile loop's) or none (a sequence with rows and no positions)."""
+    text = _code(os.path.join(CSRC, "paged_attention.cu"))
+    (math,) = [b for b in _blocks(text, r"while \(segment\(g\)\) \{")]
+    at = math.index("sums[warp * ROWS")
+    (with_tiles,) = _blocks(math[:at], r"for \(uint32_t t = g\.t0; t < g\.t1; \+\+t, \+\+it\) \{")
+    assert "bar_math();" in with_tiles
+    (head,) = _blocks(math[:at], r"if \(MT == 1 && g\.t0 < g\.t1\) \{")
+    behind = math[math.index(head) + len(head):at].lstrip("} \n")
+    assert behind.startswith("else {") and behind[len("else {"):].lstrip().startswith("bar_math();")
