@@ -253,8 +253,8 @@ __global__ void __launch_bounds__(1024) logits_rules_kernel(const __grid_constan
         if (out) *reinterpret_cast<Pack *>(out + t) = p[k];
       }
     }
-    // Where the largest lies is looked for only when it is above all that the warp has seen.
-    const uint32_t key = __float_as_uint(most) ^ ((uint32_t)((int)__float_as_uint(most) >> 31) | 0x80000000u), highest = __reduce_max_sync(0xffffffffu, key);
+    // Where the largest lies is looked for only when it is above all that the warp has seen.  Both zeros are one value: -0 + 0 = +0.
+    const uint32_t bits = __float_as_uint(__fadd_rn(most, 0.f)), key = bits ^ ((uint32_t)((int)bits >> 31) | 0x80000000u), highest = __reduce_max_sync(0xffffffffu, key);
     if (highest > above) {
       above = highest;
       if (key == highest) {
