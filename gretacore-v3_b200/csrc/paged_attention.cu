@@ -11,6 +11,9 @@
 // fp32 queries and probabilities travel as two fp16 or three bf16 values each (of the cache's type, which is exact), products are exact in the fp32
 // accumulators: 22 or 24 bits are kept.  16-bit queries are used as they are, probabilities are rounded to 16 bits (half a step: 2^-11 or 2^-8 of each, the sum of
 // them is taken in fp32 of the unrounded values).
+// fp16 has no steps below 2^-24: probabilities are made 2^15 times as large for it (sums too, so the division at the end takes it out).  Weights down to 2^-18 of a row's
+// largest keep 22 bits then, single ones down to 2^-29 their 11, and what is smaller is off by at most 2^-40 of the largest.  (4096 keys behind one of no value and a score 12 or 14
+// higher, error of fp32 calls of the outputs' size: 5.8e-7 and 7.0e-7; with probabilities of their own size 3.2e-4 and 1.9e-3.)
 //
 // 16 sequences around 4096 positions, 64 heads over 8 of 128, fp32 queries: 58.5 us (4.6 TB/s); 32 of 4000: 92.5 us (5.7 TB/s); one sequence of 577, 32 heads: 12.9 us.
 // In front of the stream lie 2 us until the shares are known and 4.5 until the first tiles are in (table entry, then page, from all SMs at once), behind it 4 of
@@ -97,6 +100,9 @@ struct PmShape {
   static constexpr uint32_t MAXIMA = PM_WARPS * ROWS * 4;
   static constexpr size_t bytes(uint32_t batch) { return 1024 + RING + Q + QR + P + 2 * MAXIMA + ROWS * 4 + (size_t)batch * 24 + 8 + (2 * STAGES + 1) * 8 + 16; }
 };
+
+template <bool BF16>
+constexpr float PM_GAIN = BF16 ? 1.f : 32768.f;  // of probabilities; the largest, 2^15, and its sums with values fit
 
 // Tiles of a sequence's lists (all row blocks alike: those in front of a block's window or behind its last row are passed over), its blocks.
 __device__ __forceinline__ void seq_tiles(const PagedSeq &s, uint32_t group, uint32_t rows, uint32_t window, uint32_t &tile0, uint32_t &tiles, uint32_t &blocks) {
@@ -464,7 +470,7 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
             }
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-              const float p0 = ex2(s[m][n][2 * c] - nm), p1 = ex2(s[m][n][2 * c + 1] - nm);
+              const float p0 = PM_GAIN<BF16> * ex2(s[m][n][2 * c] - nm), p1 = PM_GAIN<BF16> * ex2(s[m][n][2 * c + 1] - nm);
               l[m][c] += p0 + p1;
               uint32_t v[TERMS];
               split<BF16, TERMS>(p0, p1, v);
@@ -547,7 +553,7 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
 #pragma unroll
             for (int n = 0; n < (int)DH / 16; ++n) y[n] = o[m][n / 2][2 * c + (n & 1)];
             paged_again<DH / 16>(w, BF16, F32, g.b, g.s, g.g, g.R0 + r, [&](int n) { return warp * (DH / 4) + n / 2 * 8 + 2 * t4 + (n & 1); },
-                                 max(lim0[m][c], (int)(g.t0 * PM_KEYS)), min(lim1[m][c], (int)(g.t1 * PM_KEYS)), mx[m][c], y);
+                                 max(lim0[m][c], (int)(g.t0 * PM_KEYS)), min(lim1[m][c], (int)(g.t1 * PM_KEYS)), mx[m][c], PM_GAIN<BF16>, y);
 #pragma unroll
             for (int n = 0; n < (int)DH / 16; ++n) o[m][n / 2][2 * c + (n & 1)] = y[n];
           }

@@ -33,12 +33,12 @@ bool paged_tc_fits(const PagedAttnArgs &w);
 int paged_attn_tc(cudaStream_t stream, PagedAttnArgs &w, uint32_t heads);  // paged_attention_tc.cu
 
 #ifdef __CUDACC__
-// Elements elem(0 .. N - 1) of row R's unnormalised output over the keys k0 .. k1 - 1 (all seen by the row), whose scores are taken against mx: again, where the
+// Elements elem(0 .. N - 1) of row R's unnormalised output over the keys k0 .. k1 - 1 (all seen by the row), whose scores are taken against mx and weights are `gain` times as large: again, where the
 // product with hidden keys' values left no finite numbers.  An element stays as it was if a value that the row sees is none either.  Rare and slow: a key at a time, by one
 // thread.  Inlined, and its arrays in local memory: around a call the caller's loops would keep their sums there.  Not for rows whose sum of weights is no finite number: their outputs are none whatever the values are.
 template <int N, typename Elem>
 __device__ __forceinline__ void paged_again(const PagedAttnArgs &w, bool bf16, bool f32, uint32_t b, const PagedSeq &s, uint32_t g, uint32_t R, Elem elem, int k0, int k1, float mx,
-                                         float (&y)[N]) {
+                                         float gain, float (&y)[N]) {
   const uint32_t d = w.c.dim;
   const int32_t *table = w.c.table + (size_t)b * w.c.ld_table;
   auto value = [&](const void *p, size_t i) {
@@ -71,7 +71,7 @@ __device__ __forceinline__ void paged_again(const PagedAttnArgs &w, bool bf16, b
     float t = 0.f;
 #pragma unroll 2
     for (uint32_t i = 0; i < d; ++i) t = fmaf(f32 ? static_cast<const float *>(w.q)[qi + i] : value(w.q, qi + i), value(w.c.k, row + i), t);
-    const float p = exp2f(t * w.scale2 - mx);
+    const float p = gain * exp2f(t * w.scale2 - mx);
 #pragma unroll 1
     for (int n = 0; n < N; ++n)
       if (again >> n & 1) acc[n] = fmaf(p, value(w.c.v, row + elem(n)), acc[n]);

@@ -828,7 +828,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
             for (int j = 0; j < 32; ++j) x[j] = y[j];
             paged_again<32>(w, BF16, false, g->b, g->s, g->g, (g->k.token0 + i * TT) * group + row, [&](int j) { return c + j; }, max(w.window ? pos - (int)w.window + 1 : 0, (int)(lo * PT_KEYS)),
-                            min(pos + 1, (int)((lo + n) * PT_KEYS)), m2, x);
+                            min(pos + 1, (int)((lo + n) * PT_KEYS)), m2, 1.f, x);
 #pragma unroll
             for (int j = 0; j < 32; ++j) y[j] = x[j];
           }

@@ -53,3 +53,53 @@ def test_zeros_of_both_signs_are_one_value(g, t, M, V, hist):
         for m in range(M):
             g.check(g.cuda().greta_cuda_argmax(None, rows.ptr + m * c.ld * 4, V, one.ptr))
             assert one.download(np.int32)[0] == first[m]
+
+
+def check_sink(cache, qt, rows, nats, n=4097, H=8, G=2, window=0):
+    """A first key of no value whose score is `nats` above all others', alike in a head: what a row's outputs are made of hangs far below its largest weight, and a weight's
+    rounding does not average out."""
+    d, page = 64, 32
+    bt = P.Batch([(rows, n)], H, G, d, page, cache, seed=rows)
+    k = np.zeros((n, G, d))
+    k[:, :, 0] = 20 - nats
+    k[0, :, 0] = 20
+    v = bt.rng.normal(2, 1, (n, G, d))
+    v[0] = 0
+    p = np.arange(n)
+    bt.k[bt.table[0, p // page], :, p % page] = P.to_type(k, cache).view(np.uint16)
+    bt.v[bt.table[0, p // page], :, p % page] = P.to_type(v, cache).view(np.uint16)
+    bt.upload()
+    q64 = np.zeros((rows, H, d))
+    q64[:, :, 0] = 8 - np.arange(H) / 8  # exact, as its products with the keys are
+    got = P.to_f64(P.run_attention(bt, P.to_type(q64, qt), qt, scale=0.125), qt)
+    want, mag = P.attention64(bt, q64, scale=0.125)
+    # In powers of two: scores up to X are rounded as they are scaled, and their largest, by the scale's 2^-23 of their distance D and in the subtraction.  Exponential and split: 2^-22 each.
+    X, D, one = 20 * 1.4427, nats * 1.4427, 2.0 ** -24
+    weight = np.log(2) * one * (3 * D + 2 * X) + 2.0 ** -21
+    # Sums: a tile of 64 keys to the next, of weights and of outputs; within one four products of every term and eight sums.
+    sums = (2 * n / 64 + 32) * one
+    least = 2.0 ** -40 if cache == "f16" else 0.0  # of the largest weight: where fp16's steps end
+    if qt != "f32":  # probabilities of 16 bits, at least 2^7 times as large as the weight against the row's largest
+        weight, least = weight + P.HALF[qt], 2.0 ** -32 if cache == "f16" else 0.0
+    seen = np.abs(P.to_f64(P.to_type(v, cache), cache)).sum(0).max()
+    tol = mag * (2 * weight + sums) + least * seen + np.abs(want) * P.HALF[qt]  # the sum of weights is above 1
+    worst = float((np.abs(got - want) / tol).max())
+    assert worst <= 1, worst
+
+
+@pytest.mark.parametrize("nats", [8, 10, 12, 14, 18])
+@pytest.mark.parametrize("cache,qt,rows", [("f16", "f32", 1), ("bf16", "f32", 1), ("f16", "f32", 5), ("bf16", "f32", 5), ("f16", "f32", 200), ("f16", "f16", 1), ("bf16", "bf16", 1)])
+def test_outputs_that_hang_on_small_weights(g, cache, qt, rows, nats):
+    check_sink(cache, qt, rows, nats)
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+@pytest.mark.parametrize("specs,H,G", [([(1, 4096)] * 4, 16, 2), ([(1, 20011)], 5, 1), ([(40, 4096)], 4, 2)])
+def test_fp32_calls_over_long_lists_keep_fp32_precision(g, cache, specs, H, G):
+    """By the root of the mean square.  Weights of one 16-bit value would leave 1e-4 and more; sums kept in the tensor core's accumulators 4e-6."""
+    bt = P.Batch(specs, H, G, 128, 64, cache, seed=43)
+    bt.upload()
+    q = P.random_queries(bt, "f32")
+    want, _ = P.attention64(bt, q.astype(np.float64))
+    got = P.run_attention(bt, q, "f32").astype(np.float64)
+    assert np.sqrt(((got - want) ** 2).mean() / (want ** 2).mean()) <= 2e-6
