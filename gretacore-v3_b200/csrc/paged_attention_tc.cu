@@ -7,9 +7,11 @@
 //   second tile, two threads each (64 keys of a tile, half of the outputs): maxima, probabilities, outputs.
 // The two tiles take turns: while the tensor core multiplies one (P V of this key tile, Q K of the next), the other's probabilities are made.
 //   tensor memory: scores of tile A and B at columns 0 and 128, each half of which is overwritten by its probabilities (32 columns), outputs at 256 and 384.
-// A row's sums are rescaled only when its maximum has grown by more than 2^8 (probabilities up to 2^8 fit every type); the scores' barrier of a key tile says that
+// A row's sums are rescaled only when its maximum has grown by more than 2^8; the scores' barrier of a key tile says that
 // the products of the one before are in, so the rows' own threads do that.
-// Probabilities are rounded to the cache's type for the second product (half a step: 2^-11 or 2^-8 of each); the sum of them is taken in fp32 before that.
+// Probabilities are rounded to the cache's type for the second product (half a step: 2^-11 or 2^-8 of each); the sum of them is taken in fp32 before that.  fp16's steps end at
+// 2^-24, so they are taken against the maximum less 7 there: up to 2^15, sums as well, and the division at the end takes it out.  Weights down to 2^-21 of a row's largest keep their 11 bits
+// (4096 keys behind one of no value and a score 14 higher: error 3.5e-4 of the outputs' size, without 3.5e-3).
 //
 // What bounds it: the tensor core (58 % of the time) and the exponentials (special-function unit 59 %, 16 cycles a warp in any type) take turns that do not overlap whole; every
 // row's 64 scores, bounds and sums take the 96 registers that 18 warps leave a thread (a spill in this loop goes to the second-level cache, since tiles leave the first 28 KB:
@@ -39,6 +41,8 @@ constexpr uint32_t PT_BARRIERS = 28, PT_SMALL = 3328;  // of a CTA; bytes of sha
 constexpr uint32_t PT_SLAB = 128 * 128;  // bytes of 64 elements of 128 rows
 constexpr float PT_LAZY = 8.f;           // log2 of what a row's maximum may grow by before its sums are rescaled
 constexpr float PT_LOWEST = -3.4028234e38f;  // a row's maximum before any score
+template <bool BF16>
+constexpr float PT_BELOW = BF16 ? 0.f : 7.f;  // m2 is this much (log2) below the maximum that it stands for
 
 __device__ __forceinline__ void tma_load_3d(void *smem_dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(smem_u32(smem_dst)),
@@ -655,7 +659,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
       const uint32_t of_half = g32 + i * 4;
       const uint32_t tokens = lds(of_half + offsetof(Segment, k.tokens)), lo = lds(of_half + offsetof(Segment, k.lo)), n = lds(of_half + offsetof(Segment, k.hi)) - lo;
       const bool any_live = quad * 32 < tokens * group;
-      float m2 = PT_LOWEST, l = 0.f;  // the row's maximum times scale2; the sum of this thread's half
+      float m2 = PT_LOWEST, l = 0.f;  // the row's maximum times scale2, less PT_BELOW; the sum of this thread's half
       // What a tile needs of the segment is read from shared memory where it is needed: the row's scores leave no registers for it.
       for (uint32_t t = lo; t < lo + n; ++t) {  // to the end, whatever became of a wait: the two warps of a row meet in every tile
         if (ok) ok = __all_sync(0xffffffffu, poll(sm + (SF + i) * 8, phases & 1, sm + ABORT, 960 + i));
@@ -724,10 +728,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         const float tmax = fmaxf(largest(v), largest(u));
         float sum = 0.f;
         if (!start) sum = probabilities(v, sb + 32);
-        if (agree(start || tmax * w.scale2 > m2 + PT_LAZY)) {
+        if (agree(start || tmax * w.scale2 > m2 + (PT_LAZY + PT_BELOW<BF16>))) {
           sts(mine, __float_as_uint(tmax));
           meet_other();
-          const float nm = fmaxf(m2, fmaxf(tmax, __uint_as_float(lds(theirs))) * w.scale2);
+          const float nm = fmaxf(m2, fmaxf(tmax, __uint_as_float(lds(theirs))) * w.scale2 - PT_BELOW<BF16>);
           const bool grown = start || nm > m2 + PT_LAZY;
           const float f = grown ? ex2(m2 - nm) : 1.f;
           if (grown) m2 = nm;

@@ -93,6 +93,12 @@ def test_outputs_that_hang_on_small_weights(g, cache, qt, rows, nats):
     check_sink(cache, qt, rows, nats)
 
 
+@pytest.mark.parametrize("nats", [8, 10, 12, 14, 18])
+@pytest.mark.parametrize("cache,rows", [("f16", 5), ("f16", 200), ("bf16", 200), ("f16", 700)])
+def test_outputs_of_portions_that_hang_on_small_weights(g, cache, rows, nats):
+    check_sink(cache, cache, rows, nats)
+
+
 @pytest.mark.parametrize("cache", ["f16", "bf16"])
 @pytest.mark.parametrize("specs,H,G", [([(1, 4096)] * 4, 16, 2), ([(1, 20011)], 5, 1), ([(40, 4096)], 4, 2)])
 def test_fp32_calls_over_long_lists_keep_fp32_precision(g, cache, specs, H, G):
