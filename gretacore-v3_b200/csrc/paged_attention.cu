@@ -290,8 +290,9 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
         if (F32) return __ldcg(reinterpret_cast<const float2 *>(static_cast<const float *>(w.q) + i));
         return unpack2<BF16>(__ldcg(reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(w.q) + i)));
       };
-      // fp32 rows are divided by the power of two in front of their largest element, whatever it is, so that their terms keep their bits.
-      auto down = [&](float most) { return most > 0.f && most < INFINITY ? exp2f(-(float)max(-100, min(100, ilogbf(most)))) : 1.f; };
+      // fp32 rows are divided by the power of two in front of their largest element, whatever it is, so that their terms keep their bits; in fp16, whose steps end at 2^-24, they
+      // are brought to 2^14, and elements down to 2^-17 of the largest keep 22 bits.
+      auto down = [&](float most) { return most > 0.f && most < INFINITY ? exp2f((BF16 ? 0.f : 14.f) - (float)max(-100, min(100, ilogbf(most)))) : 1.f; };
       if (MT == 1 && g.t0 < g.t1) {
         if (ok) ok = mbar_wait_now(&full[it % STAGES], (it / STAGES) & 1, abort_flag, 815);
         ok = __all_sync(0xffffffffu, ok);

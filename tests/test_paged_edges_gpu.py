@@ -109,3 +109,25 @@ def test_fp32_calls_over_long_lists_keep_fp32_precision(g, cache, specs, H, G):
     want, _ = P.attention64(bt, q.astype(np.float64))
     got = P.run_attention(bt, q, "f32").astype(np.float64)
     assert np.sqrt(((got - want) ** 2).mean() / (want ** 2).mean()) <= 2e-6
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+@pytest.mark.parametrize("far", [6, 10, 14])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_small_elements_beside_a_large_one(g, cache, far, rows):
+    """fp32 queries whose largest element meets keys of zero there: scores are made of an element that is 2^-far of it, as exactly as if it stood alone."""
+    n, H, G, d, page = 500, 4, 2, 64, 32
+    bt = P.Batch([(rows, n)], H, G, d, page, cache, seed=61)
+    k = np.zeros((n, G, d))
+    k[:, :, 1] = np.round(bt.rng.uniform(-64, 64, (n, G)))  # exact in both types
+    p = np.arange(n)
+    bt.k[bt.table[0, p // page], :, p % page] = P.to_type(k, cache).view(np.uint16)
+    bt.upload()
+    q = np.zeros((rows, H, d), np.float32)
+    q[:, :, 1] = bt.rng.uniform(1, 2, (rows, H))
+    q[:, :, 0] = 2.0 ** far
+    got = P.run_attention(bt, q, "f32", scale=0.125).astype(np.float64)
+    want, mag = P.attention64(bt, q.astype(np.float64), scale=0.125)
+    # Scores up to 16: the element by 2^-22 in its terms, two sums, the scale's 2^-23 and one rounding more; of a score and of the largest one.  Exponential and split 2^-22 each, sums of eight tiles.
+    weight = 2 * 16 * (2.0 ** -22 + 4 * 2.0 ** -23) + 2.0 ** -21
+    assert (np.abs(got - want) <= mag * (2 * weight + 48 * 2.0 ** -24) + 1e-9).all()
