@@ -81,7 +81,7 @@ __device__ __forceinline__ bool test(uint32_t bar, uint32_t parity) {  // at onc
   return ok != 0;
 }
 // No call: what a caller's registers hold would go to local memory around it, and come back from the second-level cache when the wait is over.
-__device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity, uint32_t abort_flag, int code) {
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t abort_flag, int code) {
   if (try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   bool ok;
@@ -91,7 +91,6 @@ __device__ __forceinline__ bool poll(uint32_t bar, uint32_t parity, uint32_t abo
   } while (!ok && !lds(abort_flag));
   return ok;
 }
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_t abort_flag, int code) { return poll(bar, parity, abort_flag, code); }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if (!BF16) return half2_bits(a, b);
@@ -415,7 +414,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
   uint32_t had = 0;
   auto next = [&](bool &ok, auto together) -> uint32_t {  // its address, 0: there is none
     const uint32_t x = had & 1, at = sm + SEGMENTS + x * (uint32_t)sizeof(Segment);
-    if (ok) ok = __all_sync(0xffffffffu, poll(sm + (NF + x) * 8, had >> 1 & 1, sm + ABORT, 980 + x));
+    if (ok) ok = __all_sync(0xffffffffu, mbar_wait(sm + (NF + x) * 8, had >> 1 & 1, sm + ABORT, 980 + x));
     ok = together(ok);
     return ok && lds(at + offsetof(Segment, more)) ? at : 0;
   };
@@ -561,7 +560,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
           constexpr uint32_t i = I.value;
           if (vt && t - 1 >= h.lo && t - 1 < h.hi) {
             if (!have_v) {
-              if (ok) ok = poll(sm + (FULL + sv) * 8, (iv / PT_UNITS) & 1, sm + ABORT, 920);
+              if (ok) ok = mbar_wait(sm + (FULL + sv) * 8, (iv / PT_UNITS) & 1, sm + ABORT, 920);
+              __syncwarp();
               have_v = true;
               if (tail && t == t1) {  // what the last page holds behind the sequence's end: zeros
                 const uint32_t pieces = tail * 8, from = smem_u32(ring) + sv * UNIT + (PT_KEYS - tail) * 128;
@@ -573,7 +573,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
             }
 #pragma unroll
             for (uint32_t part = 0; part < 2; ++part) {
-              if (ok) ok = poll(sm + (PF + 2 * i + part) * 8, h.tiles & 1, sm + ABORT, 930 + 2 * i + part);
+              if (ok) ok = mbar_wait(sm + (PF + 2 * i + part) * 8, h.tiles & 1, sm + ABORT, 930 + 2 * i + part);
               __syncwarp();
               if (leader && ok) {
                 tc_fence_after();
@@ -593,11 +593,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
           }
           if (kt && t >= h.lo && t < h.hi) {
             if (!have_k) {
-              if (ok) ok = poll(sm + (FULL + sk) * 8, (ik / PT_UNITS) & 1, sm + ABORT, 940);
+              if (ok) ok = mbar_wait(sm + (FULL + sk) * 8, (ik / PT_UNITS) & 1, sm + ABORT, 940);
+              __syncwarp();
               have_k = true;
             }
             if (t == h.lo) {
-              if (ok) ok = poll(sm + (QF + i) * 8, h.loads & 1, sm + ABORT, 910 + i);
+              if (ok) ok = mbar_wait(sm + (QF + i) * 8, h.loads & 1, sm + ABORT, 910 + i);
+              __syncwarp();
             }
             __syncwarp();
             if (leader && ok) {
@@ -662,7 +664,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
       float m2 = PT_LOWEST, l = 0.f;  // the row's maximum times scale2, less PT_BELOW; the sum of this thread's half
       // What a tile needs of the segment is read from shared memory where it is needed: the row's scores leave no registers for it.
       for (uint32_t t = lo; t < lo + n; ++t) {  // to the end, whatever became of a wait: the two warps of a row meet in every tile
-        if (ok) ok = __all_sync(0xffffffffu, poll(sm + (SF + i) * 8, phases & 1, sm + ABORT, 960 + i));
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(sm + (SF + i) * 8, phases & 1, sm + ABORT, 960 + i));
         phases ^= 1;
         tc_fence_after();
         if (!any_live) {  // rows behind the last: their probabilities may be anything
@@ -758,7 +760,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
         release(1);
       }
       if (n) {
-        if (ok) ok = __all_sync(0xffffffffu, poll(sm + (FIN + i) * 8, phases >> 1 & 1, sm + ABORT, 970 + i));
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(sm + (FIN + i) * 8, phases >> 1 & 1, sm + ABORT, 970 + i));
         phases ^= 2;
       }
       if (any_live) {

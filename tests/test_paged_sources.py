@@ -1,7 +1,10 @@
 """Rules of the paged operators' sources that no run shows reliably."""
 import os
+import re
 
-from test_kernel_sources import CSRC, _blocks, _code
+import pytest
+
+from test_kernel_sources import CSRC, ELECTING, _blocks, _code
 
 
 def test_sums_of_a_row_block_are_read_before_the_next_are_written():
@@ -15,3 +18,14 @@ def test_sums_of_a_row_block_are_read_before_the_next_are_written():
     (head,) = _blocks(math[:at], r"if \(MT == 1 && g\.t0 < g\.t1\) \{")
     behind = math[math.index(head) + len(head):at].lstrip("} \n")
     assert behind.startswith("else {") and behind[len("else {"):].lstrip().startswith("bar_math();")
+
+
+@pytest.mark.parametrize("name", ELECTING)
+def test_what_waits_for_a_barrier_is_called_so(name):
+    """The rule that lanes meet between a wait and an issue looks for waits by their name: a function of an issuing kernel's source that loops on a barrier's phase has no other."""
+    text = _code(os.path.join(CSRC, name))
+    for m in re.finditer(r"\bbool (\w+)\([^)]*\) \{", text):
+        if "try_wait(" in next(_blocks(text[m.start():], r"\) \{")):
+            assert m.group(1).startswith("mbar_wait"), m.group(1)
+    for m in re.finditer(r"\bbool (\w+)\([^)]*\) \{\s*return (\w+)\(", text):
+        assert not m.group(2).startswith("mbar_wait") or m.group(1).startswith("mbar_wait"), m.group(1)
