@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "greta_cuda.h"
 
 namespace greta {
@@ -106,6 +108,24 @@ inline cudaError_t launch_pdl_cluster(void (*kernel)(KArgs...), dim3 grid, dim3 
 }
 
 inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Whether one of n rows of wa bytes, pa apart, shares a byte with one of n rows of wb bytes, pb apart.  Rows of two tensors may lie between each other (columns of one buffer).
+inline bool rows_meet(const void *a, size_t pa, size_t wa, const void *b, size_t pb, size_t wb, size_t n) {
+  if (n == 0) return false;
+  const int64_t d = (int64_t)(reinterpret_cast<uintptr_t>(b) - reinterpret_cast<uintptr_t>(a)), A = (int64_t)pa, B = (int64_t)pb, u = (int64_t)wa, v = (int64_t)wb, last = (int64_t)n - 1;
+  auto behind = [](int64_t x, int64_t step) { return (x >= 0 ? x / step : -((-x + step - 1) / step)) + 1; };  // the first multiple above x
+  // row j of b meets row i of a where i A - v < d + j B < i A + u
+  if (d >= last * A + u || d + last * B + v <= 0) return false;
+  if (A == B) {
+    const int64_t k = std::max(behind(-v - d, B), -last);  // j - i
+    return k <= last && d + k * B < u;
+  }
+  for (int64_t i = 0; i <= last; ++i) {
+    const int64_t j = std::max(behind(i * A - v - d, B), (int64_t)0);
+    if (j <= last && d + j * B < i * A + u) return true;
+  }
+  return false;
+}
 
 // Payload bytes per block of 32 weights in the qs plane; 0 for unknown formats.
 __host__ __device__ constexpr int payload_bytes(int fmt) {

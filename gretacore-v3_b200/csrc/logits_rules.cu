@@ -392,6 +392,7 @@ int adjust(greta_stream_t stream, const greta_logits_rules *rules, int fmt, cons
   GRETA_REQUIRE(!advance || (d_next && rules->ids), "%s: nothing to append to", name);
   const uint32_t size = fmt == GRETA_FMT_F32 ? 4 : 2;
   GRETA_REQUIRE((uintptr_t)logits % size == 0 && (uintptr_t)out % size == 0, "%s: misaligned pointer", name);
+  GRETA_REQUIRE(!out || out == logits || !rows_meet(logits, (size_t)ld * size, (size_t)V * size, out, (size_t)ld_out * size, (size_t)V * size, M), "%s: out overlaps the logits", name);
   LogitsArgs a{};
   a.r = *rules;
   a.in = logits;

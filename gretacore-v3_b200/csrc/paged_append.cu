@@ -300,6 +300,10 @@ extern "C" int greta_cuda_paged_append(greta_stream_t stream, const greta_paged_
     const long double scaled = part * 18446744073709551616.0L + 0.5L;
     a.turn[i] = scaled >= 18446744073709551616.0L ? 0 : (uint64_t)scaled;
   }
+  auto over = [&](const void *p, uint32_t ld, uint32_t n) {
+    return rows_meet(p, (size_t)ld * paged_size(fmt), (size_t)n * d * paged_size(fmt), q_out, (size_t)ld_q_out * paged_size(q_fmt), (size_t)heads * d * paged_size(q_fmt), rows->tokens);
+  };
+  GRETA_REQUIRE(!q || !((q != q_out && over(q, ld_q, heads)) || over(k, ld_k, G) || over(v, ld_v, G)), "paged_append: q_out overlaps q, k or v");
   if (rows->tokens == 0) return GRETA_OK;
   // Few tokens: heads spread over more CTAs, down to a unit or two per thread.
   const bool vec = a.dims % 16 == 0;

@@ -710,6 +710,8 @@ int greta_cuda_paged_attn(greta_stream_t stream, const greta_paged_cache *cache,
   GRETA_REQUIRE(window < (1u << 31) && scale > 0 && isfinite(scale), "paged_attn: window %u, scale %g", window, scale);
   GRETA_REQUIRE(aligned16(workspace) && workspace_bytes >= greta_cuda_paged_attn_workspace_bytes(d), "paged_attn: workspace of %zu bytes, %zu needed", workspace_bytes,
                 greta_cuda_paged_attn_workspace_bytes(d));
+  const size_t row = (size_t)heads * d * paged_size(q_fmt);
+  GRETA_REQUIRE(!rows_meet(q, (size_t)ld_q * paged_size(q_fmt), row, o, (size_t)ld_o * paged_size(q_fmt), row, rows->tokens), "paged_attn: o overlaps q");
   if (rows->tokens == 0) return GRETA_OK;
   EncodeTiledFn enc = encode_tiled();
   if (!enc) {

@@ -465,7 +465,7 @@ typedef struct greta_rotation {
   float amplitude;
 } greta_rotation;
 /* New rows of q [tokens][heads][dim], k and v [tokens][kv_heads][dim], all of type fmt (GRETA_FMT_F32, F16 or BF16): k rotated to the
- * cache, v to the cache, q rotated to q_out (type q_fmt, any of the three; q_out may be q where types and ld agree).  q and q_out may
+ * cache, v to the cache, q rotated to q_out (type q_fmt, any of the three; q_out may be q where types and ld agree, and overlaps q, k and v in no other way).  q and q_out may
  * be NULL together.  ld_*: elements from a token to the next.  Pointers 16-byte aligned, ld_* whole 16 bytes.  The ragged form of greta_cuda_rope_kv
  * (launch_rope and launch_kv_update, attention_kernels.hip:28-158).  Two rows of one call at the same place of the cache: either is kept. */
 GRETA_API int greta_cuda_paged_append(greta_stream_t stream, const greta_paged_cache *cache, const greta_ragged *rows, const greta_rotation *rotation, int fmt,
@@ -502,7 +502,7 @@ typedef struct greta_logits_rules {
   const uint32_t *allowed;    /* [M][ld_allowed] */
   uint32_t ld_allowed;        /* words, at least V / 32 rounded up */
 } greta_logits_rules;
-/* out = the logits under the rules (type fmt: GRETA_FMT_F32, F16 or BF16, rounded once; may be the logits themselves, with the same ld; NULL:
+/* out = the logits under the rules (type fmt: GRETA_FMT_F32, F16 or BF16, rounded once; may be the logits themselves, with the same ld, and overlaps them in no other way; NULL:
  * not wanted), d_next[m] = the first maximum of row m as it is written (greta_cuda_argmax's rules; NULL: not wanted).  ld, ld_out: elements between rows.  Stands in front of,
  * or in the place of, launch_argmax (basic_kernels.hip:330-373). */
 GRETA_API int greta_cuda_logits_adjust(greta_stream_t stream, const greta_logits_rules *rules, int fmt, const void *logits, uint32_t ld, void *out,

@@ -131,3 +131,35 @@ def test_small_elements_beside_a_large_one(g, cache, far, rows):
     # Scores up to 16: the element by 2^-22 in its terms, two sums, the scale's 2^-23 and one rounding more; of a score and of the largest one.  Exponential and split 2^-22 each, sums of eight tiles.
     weight = 2 * 16 * (2.0 ** -22 + 4 * 2.0 ** -23) + 2.0 ** -21
     assert (np.abs(got - want) <= mag * (2 * weight + 48 * 2.0 ** -24) + 1e-9).all()
+
+
+def test_rows_of_several_tensors_in_one_buffer(g):
+    """Queries, keys, values, rotated queries and outputs as columns of one buffer, and logits beside what is made of them."""
+    lib, T, H, G, d, V = g.cuda(), 6, 4, 2, 64, 40
+    bt = P.Batch([(4, 4), (2, 2)], H, G, d, 16, "f16", seed=71)
+    bt.upload()
+    widths = dict(q=H * d, k=G * d, v=G * d, turned=H * d, o=H * d, logits=V, out=V)
+    at, ld = {}, 0
+    for name, n in widths.items():
+        at[name], ld = ld, ld + n
+    rng = np.random.default_rng(72)
+    x = rng.normal(0, 1, (T, ld)).astype(np.float32)
+    buf = P.device(x)
+    p = lambda name: buf.ptr + 4 * at[name]
+    c, r = bt.structs()
+    rot = g.Rotation(dims=d, interleaved=0, base=10000.0, freq=None, amplitude=1.0)
+    ws = g.DeviceBuffer(lib.greta_cuda_paged_attn_workspace_bytes(d), zero=True)
+    g.check(lib.greta_cuda_paged_append(None, C.byref(c), C.byref(r), C.byref(rot), 0, p("q"), ld, p("k"), ld, p("v"), ld, H, p("turned"), 0, ld))
+    g.check(lib.greta_cuda_paged_append(None, C.byref(c), C.byref(r), C.byref(rot), 0, p("q"), ld, p("k"), ld, p("v"), ld, H, p("q"), 0, ld))  # in place between the others
+    g.check(lib.greta_cuda_paged_attn(None, C.byref(c), C.byref(r), p("turned"), 0, ld, p("o"), ld, H, 0.125, 0, ws.ptr, ws.nbytes))
+    g.check(lib.greta_cuda_logits_adjust(None, C.byref(g.LogitsRules()), 0, p("logits"), ld, p("out"), ld, T, V, None))
+    y = buf.download(np.float32).reshape(T, ld)
+    col = lambda a, name: a[:, at[name]:at[name] + widths[name]]
+    for name in ("k", "v", "logits"):
+        assert np.array_equal(col(y, name), col(x, name))
+    assert np.array_equal(col(y, "out"), col(x, "logits")) and np.array_equal(col(y, "q"), col(y, "turned"))
+    for pool, name in ((bt.dk, "k"), (bt.dv, "v")):
+        setattr(bt, name, pool.download(np.uint16).reshape(bt.k.shape))
+    q64 = col(y, "turned").reshape(T, H, d).astype(np.float64)
+    want, mag = P.attention64(bt, q64)
+    assert (np.abs(col(y, "o").reshape(T, H, d) - want) <= P.attention_tolerance(bt, q64, want, mag, "f32")).all()
