@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
             }
         }
         const int k0 = (int)(t * PM_KEYS);
-        const bool masks = k0 < whole0 || k0 + (int)PM_KEYS > whole1;
+        const bool masks = k0 < whole0 || k0 > whole1 - (int)PM_KEYS;  // no sum with k0: positions end at 2^31
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
           float tm[2] = {-INFINITY, -INFINITY};
@@ -444,7 +444,7 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
         }
         // ---- values behind the sequence's end are whatever the page held before: zeros
         const int end = min((int)g.s.len, g.s.pos0 + (int)g.s.rows);
-        if (k0 + (int)PM_KEYS > end) {
+        if (k0 > end - (int)PM_KEYS) {
           const uint32_t from = (uint32_t)max(0, end - k0);
           for (uint32_t i = tid; i < (PM_KEYS - from) * SD * 8; i += 32 * PM_WARPS) {
             const uint32_t c = i / ((PM_KEYS - from) * 8), j = i % ((PM_KEYS - from) * 8);
@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
           for (int n = 0; n < (int)DH / 32; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[m][n][j] += po[m][n][j];
-        if (k0 + (int)PM_KEYS > end) fence_proxy_async();  // the zeros are in front of the next copy
+        if (k0 > end - (int)PM_KEYS) fence_proxy_async();  // the zeros are in front of the next copy
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[st]);
       }
@@ -554,7 +554,7 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
 #pragma unroll
             for (int n = 0; n < (int)DH / 16; ++n) y[n] = o[m][n / 2][2 * c + (n & 1)];
             paged_again<DH / 16>(w, BF16, F32, g.b, g.s, g.g, g.R0 + r, [&](int n) { return warp * (DH / 4) + n / 2 * 8 + 2 * t4 + (n & 1); },
-                                 max(lim0[m][c], (int)(g.t0 * PM_KEYS)), min(lim1[m][c], (int)(g.t1 * PM_KEYS)), mx[m][c], PM_GAIN<BF16>, y);
+                                 max(lim0[m][c], (int)(g.t0 * PM_KEYS)), min(lim1[m][c], (int)min(g.t1 * PM_KEYS, 0x7fffffffu)), mx[m][c], PM_GAIN<BF16>, y);
 #pragma unroll
             for (int n = 0; n < (int)DH / 16; ++n) o[m][n / 2][2 * c + (n & 1)] = y[n];
           }

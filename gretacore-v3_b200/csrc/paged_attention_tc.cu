@@ -207,7 +207,10 @@ struct Finder {
       g.clear1[i] = first < 0 ? 0 : (uint32_t)(first + 1) / PT_KEYS;
     }
   }
-  __device__ uint32_t tail(const Segment &g) const { return g.k.t1 > g.k.t0 ? (uint32_t)max(0, (int)(g.k.t1 * PT_KEYS) - (g.s.pos0 + (int)g.s.rows)) : 0; }
+  __device__ uint32_t tail(const Segment &g) const {
+    const uint32_t end = (uint32_t)(g.s.pos0 + (int)g.s.rows), tiles = g.k.t1 * PT_KEYS;  // up to 2^31
+    return g.k.t1 > g.k.t0 && tiles > end ? tiles - end : 0;
+  }
   // A whole block by its number.
   __device__ void block(uint32_t x, Segment &g) const {
     g.b = seq_at(x);
@@ -834,7 +837,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tc_kernel(const __grid_co
 #pragma unroll
             for (int j = 0; j < 32; ++j) x[j] = y[j];
             paged_again<32>(w, BF16, false, g->b, g->s, g->g, (g->k.token0 + i * TT) * group + row, [&](int j) { return c + j; }, max(w.window ? pos - (int)w.window + 1 : 0, (int)(lo * PT_KEYS)),
-                            min(pos + 1, (int)((lo + n) * PT_KEYS)), m2, 1.f, x);
+                            min(pos + 1, (int)min((lo + n) * PT_KEYS, 0x7fffffffu)), m2, 1.f, x);
 #pragma unroll
             for (int j = 0; j < 32; ++j) y[j] = x[j];
           }

@@ -163,3 +163,36 @@ def test_rows_of_several_tensors_in_one_buffer(g):
     q64 = col(y, "turned").reshape(T, H, d).astype(np.float64)
     want, mag = P.attention64(bt, q64)
     assert (np.abs(col(y, "o").reshape(T, H, d) - want) <= P.attention_tolerance(bt, q64, want, mag, "f32")).all()
+
+
+@pytest.mark.parametrize("cache,qt,rows", [("f16", "f32", 1), ("bf16", "bf16", 1), ("f16", "f32", 40), ("f16", "f16", 40)])
+@pytest.mark.parametrize("spoilt", [False, True])
+def test_positions_up_to_the_end_of_the_range(g, cache, qt, rows, spoilt):
+    """A table for 2^31 - 8 positions, all in use, and a window over the last of them; NaN in hidden values of the last page where `spoilt`."""
+    page, d, H, G, window = 8, 64, 4, 2, 100
+    ld, near = 2 ** 28 - 1, 1024  # the last 1024 positions have pages of their own
+    bt = P.Batch([(rows, near)], H, G, d, page, cache, seed=81)
+    if spoilt:  # of the last position, which the last row alone sees
+        bt.v[bt.table[0, -1], :, page - 1, 5] = P.NAN16
+    bt.upload()
+    q = P.random_queries(bt, qt)
+    q64 = P.to_f64(q, qt)
+    if spoilt:
+        clean = bt.v.copy()
+        bt.v[bt.table[0, -1], :, page - 1, 5] = 0
+        want, mag = P.attention64(bt, q64, window)
+        tol, bt.v = P.attention_tolerance(bt, q64, want, mag, qt), clean
+    else:
+        want, mag = P.attention64(bt, q64, window)
+        tol = P.attention_tolerance(bt, q64, want, mag, qt)
+    table = g.DeviceBuffer(4 * ld)
+    table.fill(0xFF)
+    table.upload(bt.table[0, :near // page], offset=4 * (ld - near // page))
+    bt.dt, bt.dl = table, P.device(np.array([ld * page], np.uint32))
+    bt.table = np.broadcast_to(np.int32(-1), (1, ld))
+    got = P.to_f64(P.run_attention(bt, q, qt, window), qt)
+    right = np.abs(got - want) <= tol
+    if spoilt:
+        assert not np.isfinite(got[-1, :, 5]).any()
+        right[-1, :, 5] = True
+    assert right.all()
