@@ -650,17 +650,23 @@ template <int SD, bool BF16, bool F32, int MT>
 int launch_mma(cudaStream_t stream, const PagedAttnArgs &w) {
   using Z = PmShape<SD, BF16, F32, MT>;
   const size_t smem = Z::bytes(w.r.batch);
-  static int ctas[64] = {};
+  // A CTA's memory grows with the batch (24 bytes a sequence): the most sequences with which an SM holds two.
+  static int two[64] = {};  // 1 + that
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) dev = 0;
-  if (ctas[dev] == 0) {
+  if (two[dev] == 0) {
     GRETA_CUDA_TRY(cudaFuncSetAttribute(paged_mma_kernel<SD, BF16, F32, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Z::bytes(PAGED_MAX_BATCH)));
-    int n = 0;
-    GRETA_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_mma_kernel<SD, BF16, F32, MT>, PM_THREADS, Z::bytes(64)));
-    ctas[dev] = std::max(1, std::min(n, (int)PAGED_CTAS_PER_SM));
+    int most = 0;
+    for (int step = (int)PAGED_MAX_BATCH; step; step /= 2) {
+      int n = 0;
+      if (most + step <= (int)PAGED_MAX_BATCH)
+        GRETA_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, paged_mma_kernel<SD, BF16, F32, MT>, PM_THREADS, Z::bytes(most + step)));
+      if (n >= (int)PAGED_CTAS_PER_SM) most += step;
+    }
+    two[dev] = most + 1;
   }
-  const uint32_t grid = std::min<uint32_t>(PAGED_MAX_CTAS, (uint32_t)(ctas[dev] * sm_count()));
+  const uint32_t grid = std::min<uint32_t>(PAGED_MAX_CTAS, ((int)w.r.batch < two[dev] ? PAGED_CTAS_PER_SM : 1) * (uint32_t)sm_count());
   GRETA_CUDA_TRY(launch_pdl(paged_mma_kernel<SD, BF16, F32, MT>, dim3(grid), dim3(PM_THREADS), smem, stream, w));
   return launched("paged_mma_kernel");
 }

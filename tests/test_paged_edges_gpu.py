@@ -196,3 +196,8 @@ def test_positions_up_to_the_end_of_the_range(g, cache, qt, rows, spoilt):
         assert not np.isfinite(got[-1, :, 5]).any()
         right[-1, :, 5] = True
     assert right.all()
+
+
+@pytest.mark.parametrize("cache,qt,batch", [("bf16", "f32", 15), ("bf16", "f32", 17), ("f16", "f32", 111), ("f16", "f32", 112), ("f16", "f16", 378), ("bf16", "bf16", 379)])
+def test_batches_around_what_two_ctas_leave_room_for(g, cache, qt, batch):
+    P.check_attention([(1, 1 + b * 7 % 200) for b in range(batch)], 4, 2, 128, 64, cache, qt, seed=91)

@@ -29,3 +29,9 @@ def test_what_waits_for_a_barrier_is_called_so(name):
             assert m.group(1).startswith("mbar_wait"), m.group(1)
     for m in re.finditer(r"\bbool (\w+)\([^)]*\) \{\s*return (\w+)\(", text):
         assert not m.group(2).startswith("mbar_wait") or m.group(1).startswith("mbar_wait"), m.group(1)
+
+
+def test_ctas_of_the_few_row_attention_go_by_the_batch():
+    """Its shared memory grows with the batch: a launch that counts on two CTAs an SM where one fits runs in two waves of half the work each."""
+    (launch,) = _blocks(_code(os.path.join(CSRC, "paged_attention.cu")), r"int launch_mma\(cudaStream_t stream, const PagedAttnArgs &w\) \{")
+    assert not re.search(r"Z::bytes\(\d+\)", launch) and "w.r.batch" in launch[launch.index("const uint32_t grid"):]
