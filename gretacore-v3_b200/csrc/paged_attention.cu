@@ -291,8 +291,10 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
         return unpack2<BF16>(__ldcg(reinterpret_cast<const uint32_t *>(static_cast<const uint16_t *>(w.q) + i)));
       };
       // fp32 rows are divided by the power of two in front of their largest element, whatever it is, so that their terms keep their bits; in fp16, whose steps end at 2^-24, they
-      // are brought to 2^14, and elements down to 2^-17 of the largest keep 22 bits.
-      auto down = [&](float most) { return most > 0.f && most < INFINITY ? exp2f((BF16 ? 0.f : 14.f) - (float)max(-100, min(100, ilogbf(most)))) : 1.f; };
+      // are brought to 2^14, and elements down to 2^-17 of the largest keep 22 bits.  The factor itself stays between 2^-126 and 2^127.
+      auto down = [&](float most) {
+        return most > 0.f && most < INFINITY ? BF16 ? exp2f(-(float)max(-126, min(126, ilogbf(most)))) : exp2f(14.f - (float)max(-113, ilogbf(most))) : 1.f;
+      };
       if (MT == 1 && g.t0 < g.t1) {
         if (ok) ok = mbar_wait_now(&full[it % STAGES], (it / STAGES) & 1, abort_flag, 815);
         ok = __all_sync(0xffffffffu, ok);

@@ -201,3 +201,15 @@ def test_positions_up_to_the_end_of_the_range(g, cache, qt, rows, spoilt):
 @pytest.mark.parametrize("cache,qt,batch", [("bf16", "f32", 15), ("bf16", "f32", 17), ("f16", "f32", 111), ("f16", "f32", 112), ("f16", "f16", 378), ("bf16", "bf16", 379)])
 def test_batches_around_what_two_ctas_leave_room_for(g, cache, qt, batch):
     P.check_attention([(1, 1 + b * 7 % 200) for b in range(batch)], 4, 2, 128, 64, cache, qt, seed=91)
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+@pytest.mark.parametrize("size", [1e-34, 1e31, 3e36])
+def test_fp32_queries_near_the_ends_of_their_range(g, size, cache):
+    bt = P.Batch([(1, 200), (30, 90)], 4, 2, 64, 16, cache, seed=3)
+    bt.upload()
+    q = P.random_queries(bt, "f32", size)
+    scale = float(np.float32(0.125 / size))
+    got = P.run_attention(bt, q, "f32", scale=scale)
+    want, mag = P.attention64(bt, q.astype(np.float64), scale=scale)
+    assert (np.abs(got - want) <= P.attention_tolerance(bt, q.astype(np.float64), want, mag, "f32", scale=scale)).all()
