@@ -715,7 +715,8 @@ int greta_cuda_paged_attn(greta_stream_t stream, const greta_paged_cache *cache,
   GRETA_REQUIRE(aligned16(q) && aligned16(o) && (size_t)ld_q * paged_size(q_fmt) % 16 == 0 && (size_t)ld_o * paged_size(q_fmt) % 16 == 0,
                 "paged_attn: rows that do not begin at 16-byte boundaries");
   GRETA_REQUIRE(q != o, "paged_attn: in place");
-  GRETA_REQUIRE(window < (1u << 31) && scale > 0 && isfinite(scale), "paged_attn: window %u, scale %g", window, scale);
+  const float scale2 = scale * 1.4426950408889634f;  // of powers of two
+  GRETA_REQUIRE(window < (1u << 31) && scale2 > 0 && isfinite(scale2), "paged_attn: window %u, scale %g", window, scale);
   GRETA_REQUIRE(aligned16(workspace) && workspace_bytes >= greta_cuda_paged_attn_workspace_bytes(d), "paged_attn: workspace of %zu bytes, %zu needed", workspace_bytes,
                 greta_cuda_paged_attn_workspace_bytes(d));
   const size_t row = (size_t)heads * d * paged_size(q_fmt);
@@ -735,7 +736,7 @@ int greta_cuda_paged_attn(greta_stream_t stream, const greta_paged_cache *cache,
   w.ld_o = ld_o;
   w.group = heads / cache->kv_heads;
   w.window = window;
-  w.scale2 = scale * 1.4426950408889634f;
+  w.scale2 = scale2;
   w.tickets = static_cast<uint32_t *>(workspace);
   w.parts = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + PAGED_TICKETS);
   if (int rc = gemm_ts_error_word(&w.error)) return rc;

@@ -473,7 +473,7 @@ GRETA_API int greta_cuda_paged_append(greta_stream_t stream, const greta_paged_c
                                       int q_fmt, uint32_t ld_q_out);
 /* o = softmax(scale q k^T) v of every new row over the positions up to its own, with window > 0 over the last `window` of them.  q and o
  * [tokens][heads][dim], both of type q_fmt: GRETA_FMT_F32 (products and sums keep fp32 precision), or the cache's type (probabilities are
- * rounded to it, the rest is fp32).  heads: a multiple of kv_heads; scale: above 0.  The new rows' keys and values are in the cache already (greta_cuda_paged_append).  What
+ * rounded to it, the rest is fp32).  heads: a multiple of kv_heads; scale: above 0, at most 2e38.  The new rows' keys and values are in the cache already (greta_cuda_paged_append).  What
  * lies behind a row's position, or in front of its window, does not reach it whatever it is.  Rows without keys are zeros.  o and q do not overlap.
  * workspace: greta_cuda_paged_attn_workspace_bytes(dim) bytes, 16-byte aligned, its first 64 KB zero before the first call; one serves every
  * shape, one call at a time.  Waits in the kernels are bounded; one that gave up shows in greta_cuda_gemm_segments_status, and the workspace is cleared again before the

@@ -89,3 +89,12 @@ def test_adjusted_logits_over_the_logits(f, off, ld, ld_out):
     p += 4096
     assert f.cuda().greta_cuda_logits_adjust(None, C.byref(f.LogitsRules()), 0, p, ld, p + off, ld_out, 2, 100, None) == 4
     assert b"overlaps" in f.cuda().greta_cuda_last_error()
+
+
+@pytest.mark.parametrize("scale", [3e38, 2.4e38])
+def test_scales_that_leave_the_range_in_powers_of_two(f, scale):
+    buf, p = _buf()
+    cache = f.PagedCache(fmt=1, k=p, v=p, pages=4, kv_heads=2, page=16, dim=64, table=p, ld_table=4)
+    rows = f.Ragged(batch=2, tokens=3, max_rows=0, start=p, len=p)
+    assert f.cuda().greta_cuda_paged_attn(None, C.byref(cache), C.byref(rows), p, 0, 256, p + 4096, 256, 4, scale, 0, p, 1 << 40) == 4
+    assert b"scale" in f.cuda().greta_cuda_last_error()
