@@ -467,7 +467,8 @@ typedef struct greta_rotation {
 /* New rows of q [tokens][heads][dim], k and v [tokens][kv_heads][dim], all of type fmt (GRETA_FMT_F32, F16 or BF16): k rotated to the
  * cache, v to the cache, q rotated to q_out (type q_fmt, any of the three; q_out may be q where types and ld agree, and overlaps q, k and v in no other way).  q and q_out may
  * be NULL together.  ld_*: elements from a token to the next.  Pointers 16-byte aligned, ld_* whole 16 bytes.  The ragged form of greta_cuda_rope_kv
- * (launch_rope and launch_kv_update, attention_kernels.hip:28-158).  Two rows of one call at the same place of the cache: either is kept. */
+ * (launch_rope and launch_kv_update, attention_kernels.hip:28-158).  Two rows of one call at the same place of the cache (sequences that share a page):
+ * what they have alike is kept, every other element is the one's or the other's. */
 GRETA_API int greta_cuda_paged_append(greta_stream_t stream, const greta_paged_cache *cache, const greta_ragged *rows, const greta_rotation *rotation, int fmt,
                                       const void *q, uint32_t ld_q, const void *k, uint32_t ld_k, const void *v, uint32_t ld_v, uint32_t heads, void *q_out,
                                       int q_fmt, uint32_t ld_q_out);

@@ -213,3 +213,28 @@ def test_fp32_queries_near_the_ends_of_their_range(g, size, cache):
     got = P.run_attention(bt, q, "f32", scale=scale)
     want, mag = P.attention64(bt, q.astype(np.float64), scale=scale)
     assert (np.abs(got - want) <= P.attention_tolerance(bt, q.astype(np.float64), want, mag, "f32", scale=scale)).all()
+
+
+@pytest.mark.parametrize("dims", [64, 6])
+def test_appends_of_two_sequences_to_a_page_they_share(g, dims):
+    """Equal rows stay whole; of unequal ones every element is the one's or the other's."""
+    lib, T, G, d = g.cuda(), 16, 2, 64
+    bt = P.Batch([(8, 8), (8, 8)], 2, G, d, 8, "f16", seed=95)
+    bt.table[1] = bt.table[0]
+    bt.upload()
+    rng = np.random.default_rng(96)
+    c, r = bt.structs()
+    rot = g.Rotation(dims=dims, interleaved=0, base=10000.0, freq=None, amplitude=1.0)
+
+    def call(k, v):
+        dk, dv = P.device(k), P.device(v)
+        g.check(lib.greta_cuda_paged_append(None, C.byref(c), C.byref(r), C.byref(rot), 0, None, 0, dk.ptr, G * d, dv.ptr, G * d, 0, None, 0, 0))
+        g.check(lib.greta_cuda_device_synchronize())
+        return [b.download(np.uint16).reshape(bt.k.shape)[bt.table[0, 0]] for b in (bt.dk, bt.dv)]
+
+    one, two = (rng.normal(0, 1, (2, 8, G, d)).astype(np.float32) for _ in range(2))
+    alone = [call(*(np.concatenate([a, a]) for a in x)) for x in (one, two)]
+    assert np.array_equal(alone[0][1], one[1].transpose(1, 0, 2).astype(np.float16).view(np.uint16))
+    both = call(*(np.concatenate([a, b]) for a, b in zip(one, two)))
+    for got, x, y in zip(both, *alone):
+        assert ((got == x) | (got == y)).all()
