@@ -34,7 +34,7 @@ int paged_attn_tc(cudaStream_t stream, PagedAttnArgs &w, uint32_t heads);  // pa
 
 #ifdef __CUDACC__
 // Elements elem(0 .. N - 1) of row R's unnormalised output over the keys k0 .. k1 - 1 (all seen by the row), whose scores are taken against mx and weights are `gain` times as large: again, where the
-// product with hidden keys' values left no finite numbers.  An element stays as it was if a value that the row sees is none either.  Rare and slow: a key at a time, by one
+// product with hidden keys' values left no finite numbers.  Where values that the row sees are none either, they decide: their sum.  Rare and slow: a key at a time, by one
 // thread.  Inlined, and its arrays in local memory: around a call the caller's loops would keep their sums there.  Not for rows whose sum of weights is no finite number: their outputs are none whatever the values are.
 template <int N, typename Elem>
 __device__ __forceinline__ void paged_again(const PagedAttnArgs &w, bool bf16, bool f32, uint32_t b, const PagedSeq &s, uint32_t g, uint32_t R, Elem elem, int k0, int k1, float mx,
@@ -55,17 +55,27 @@ __device__ __forceinline__ void paged_again(const PagedAttnArgs &w, bool bf16, b
     return id >= 0 && (uint32_t)id < w.c.pages;
   };
   size_t row;
-  for (int j = k0; j < k1 && again; ++j) {
-    if (!row_of(j, row)) continue;
-#pragma unroll 1
-    for (int n = 0; n < N; ++n)
-      if (again >> n & 1 && !isfinite(value(w.c.v, row + elem(n)))) again &= ~(1u << n);
-  }
-  if (!again) return;
-  const size_t qi = (size_t)(s.first + R / w.group) * w.ld_q + (size_t)(g * w.group + R % w.group) * d;
   float acc[N];
 #pragma unroll 1
   for (int n = 0; n < N; ++n) acc[n] = 0.f;
+  if (!again) return;
+  for (int j = k0; j < k1; ++j) {
+    if (!row_of(j, row)) continue;
+#pragma unroll 1
+    for (int n = 0; n < N; ++n)
+      if (again >> n & 1) {
+        const float x = value(w.c.v, row + elem(n));
+        if (!isfinite(x)) acc[n] += x;
+      }
+  }
+#pragma unroll 1
+  for (int n = 0; n < N; ++n)
+    if (again >> n & 1 && acc[n] != 0.f) {
+      y[n] = acc[n];
+      again &= ~(1u << n);
+    }
+  if (!again) return;
+  const size_t qi = (size_t)(s.first + R / w.group) * w.ld_q + (size_t)(g * w.group + R % w.group) * d;
   for (int j = k0; j < k1; ++j) {
     if (!row_of(j, row)) continue;
     float t = 0.f;

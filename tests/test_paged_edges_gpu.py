@@ -238,3 +238,30 @@ def test_appends_of_two_sequences_to_a_page_they_share(g, dims):
     both = call(*(np.concatenate([a, b]) for a, b in zip(one, two)))
     for got, x, y in zip(both, *alone):
         assert ((got == x) | (got == y)).all()
+
+
+@pytest.mark.parametrize("cache,qt", [("f16", "f32"), ("bf16", "f32"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("rows,window", [(1, 0), (40, 0), (140, 0), (140, 100)])
+def test_infinities_that_a_row_sees_beside_hidden_ones(g, cache, qt, rows, window):
+    """An infinity stays one (of its sign) in the rows that see it, whatever the same element of hidden keys is; with one of the other sign, or NaN, it is NaN."""
+    n = 300
+    bt = P.Batch([(rows, n)], 4, 2, 64, 32, cache, seed=97)
+    inf = np.uint16(0x7C00 if cache == "f16" else 0x7F80)
+    spoil = [(20, 9, inf), (n - 30, 3, inf), (n - 10, 3, P.NAN16), (n - 25, 17, inf | 0x8000), (n - 5, 17, inf), (n - 28, 40, inf | 0x8000), (n - 1, 40, inf | 0x8000)]
+    for j, e, _ in spoil:
+        bt.v[bt.table[0, j // 32], :, j % 32, e] = 0
+    q = P.random_queries(bt, qt)
+    q64 = P.to_f64(q, qt)
+    want, mag = P.attention64(bt, q64, window)
+    tol = P.attention_tolerance(bt, q64, want, mag, qt)
+    pos = np.arange(n - rows, n)
+    for j, e, x in spoil:
+        bt.v[bt.table[0, j // 32], :, j % 32, e] = x
+        sees = (pos >= j) & ((pos < j + window) if window else True)
+        with np.errstate(invalid="ignore"):
+            want[sees, :, e] += np.nan if x == P.NAN16 else -np.inf if x >> 15 else np.inf
+    bt.upload()
+    got = P.to_f64(P.run_attention(bt, q, qt, window), qt)
+    odd = ~np.isfinite(want)
+    assert odd.any() and np.array_equal(got[odd], want[odd], equal_nan=True)
+    assert (np.abs(got[~odd] - want[~odd]) <= tol[~odd]).all()
