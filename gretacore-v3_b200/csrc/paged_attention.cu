@@ -392,8 +392,22 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
         uint8_t *kt = ring + (size_t)st * 2 * Z::TILE, *vt = kt + Z::TILE;
         if (ok) ok = mbar_wait_now(&full[st], (it / STAGES) & 1, abort_flag, 810 + st);
         ok = __all_sync(0xffffffffu, ok);
-        // ---- scores of the warp's 16 keys
-        float s[MT][2][4];
+        // ---- scores of the warp's 16 keys.  The tensor core cuts sums off at the accumulator's last bit, the further the more is in it: fp32 calls add two steps of 16 elements at a time to the
+        // score by an fp32 add that rounds (error of one sequence of 577 5.6e-7 -> 2.8e-7, of 16 around 4096 7.3e-7 -> 3.3e-7, the plain form's 2.2e-7 and 5.9e-7; 13.05 -> 13.15 and
+        // 59.6 -> 60.3 us, 512 rows of 4096 827 -> 883.  One step at a time: 2.5e-7 and 3.0e-7, 61.1 us.)
+        constexpr int TOGETHER = 2;
+        float s[MT][2][4], sum[MT][2][4] = {};
+        auto add = [&] {
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                sum[m][n][j] += s[m][n][j];
+                s[m][n][j] = 0.f;
+              }
+        };
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -404,6 +418,7 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
 #pragma unroll
         for (int ks = 0; ks < (int)DH / 16; ++ks) {
           uint32_t kb[4];
+          if (F32 && ks && ks % TOGETHER == 0) add();
           ldsm_x4(kb, kt + (ks / 4) * PM_KEYS * 128 + key * 128 + ((((ks & 3) * 2 + (mat & 1)) ^ (key & 7)) << 4));
 #pragma unroll
           for (int m = 0; m < MT; ++m)
@@ -429,7 +444,7 @@ __global__ void __launch_bounds__(PM_THREADS, MT == 1 ? 2 : 1) paged_mma_kernel(
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              float x = s[m][n][j] * rowf[m][j >> 1];
+              float x = (F32 ? s[m][n][j] + sum[m][n][j] : s[m][n][j]) * rowf[m][j >> 1];
               if (masks) {
                 const int k = k0 + warp * 16 + n * 8 + (int)(2 * t4) + (j & 1);
                 if (k < lim0[m][j >> 1] || k >= lim1[m][j >> 1]) x = -INFINITY;

@@ -265,3 +265,16 @@ def test_infinities_that_a_row_sees_beside_hidden_ones(g, cache, qt, rows, windo
     odd = ~np.isfinite(want)
     assert odd.any() and np.array_equal(got[odd], want[odd], equal_nan=True)
     assert (np.abs(got[~odd] - want[~odd]) <= tol[~odd]).all()
+
+
+@pytest.mark.parametrize("cache", ["f16", "bf16"])
+@pytest.mark.parametrize("specs,H,G", [([(1, 577)] * 8, 32, 32), ([(1, 4096)] * 4, 64, 8), ([(20, 577)], 32, 4)])
+def test_scores_of_fp32_calls_are_rounded_sums(g, cache, specs, H, G):
+    """By the root of the mean square 2^-21 of the outputs: about twice what 32-bit arithmetic in any order leaves.  Scores summed up in the tensor core alone, which cuts off: 5.6e-7 and more."""
+    bt = P.Batch(specs, H, G, 128, 16, cache, seed=99)
+    bt.upload()
+    q = P.random_queries(bt, "f32")
+    want, _ = P.attention64(bt, q.astype(np.float64))
+    got = P.run_attention(bt, q, "f32").astype(np.float64)
+    err = np.sqrt(((got - want) ** 2).mean() / (want ** 2).mean())
+    assert err <= 2.0 ** -21, err
