@@ -15,10 +15,12 @@
 // largest keep 22 bits then, single ones down to 2^-29 their 11, and what is smaller is off by at most 2^-40 of the largest.  (4096 keys behind one of no value and a score 12 or 14
 // higher, error of fp32 calls of the outputs' size: 5.8e-7 and 7.0e-7; with probabilities of their own size 3.2e-4 and 1.9e-3.)
 //
-// 16 sequences around 4096 positions, 64 heads over 8 of 128, fp32 queries: 58.5 us (4.6 TB/s); 32 of 4000: 92.5 us (5.7 TB/s); one sequence of 577, 32 heads: 12.9 us.
+// 16 sequences around 4096 positions, 64 heads over 8 of 128, fp32 queries: 58 us (4.7 TB/s); 32 of them: 99 us (5.4 TB/s); one sequence of 577, 32 heads: 13.0 us.
 // In front of the stream lie 2 us until the shares are known and 4.5 until the first tiles are in (table entry, then page, from all SMs at once), behind it 4 of
 // tickets and joining, and SMs are served unevenly: equal shares end 50 to 66 us after the start.  Two CTAs of three stages an SM keep 192 KB on their way; three of two do no better.
-// 64 rows a block in place of 16 for more queries: their operands come from shared memory again for every tile.
+// Where two do not fit, one keeps 96 KB: heads above 64, fp32 queries over bf16 from 16 sequences on (the third term's memory; 16 around 4096: 108 us), over fp16 from 112 (96 of 1000: 85 us,
+// 128: 165), 16 bits from 379 (128 of 1000: 95 us, 512: 506).
+// 64 rows a block in place of 16 for more queries: their operands come from shared memory again for every tile (fp32, prompt of 2048, 32 heads: 969 us over fp16, 1198 over bf16).
 #include <math.h>
 
 #include <algorithm>

@@ -13,10 +13,10 @@
 // 2^-24, so they are taken against the maximum less 7 there: up to 2^15, sums as well, and the division at the end takes it out.  Weights down to 2^-21 of a row's largest keep their 11 bits
 // (4096 keys behind one of no value and a score 14 higher: error 3.5e-4 of the outputs' size, without 3.5e-3).
 //
-// What bounds it: the tensor core (58 % of the time) and the exponentials (special-function unit 59 %, 16 cycles a warp in any type) take turns that do not overlap whole; every
+// What bounds it: the tensor core (55 % of the time) and the exponentials (special-function unit 56 %, 16 a cycle and SM in any type) take turns that do not overlap whole; every
 // row's 64 scores, bounds and sums take the 96 registers that 18 warps leave a thread (a spill in this loop goes to the second-level cache, since tiles leave the first 28 KB:
-// 58 us became 68).  512 rows behind 15872 keys, 64 heads over 8 of 128: 226 us alone (1200 TFLOP/s), 271 when the power limit has lowered the clocks; a prompt of
-// 2048, 32 heads: 45 us; of 8192: 485 (1130 TFLOP/s).
+// 58 us became 68).  512 rows behind 15872 keys, 64 heads over 8 of 128: 237 us (1150 TFLOP/s), 268 when the power limit has lowered the clocks; a prompt of
+// 2048, 32 heads: 44 us; of 8192, clocks lowered: 564 (980 TFLOP/s).
 // Blocks: where there are many, whole ones are drawn from a counter, the longest first (no joining); where drawn ones would leave SMs idle longer than joining takes, all
 // CTAs get equal shares of the places, and the last of a block's CTAs to finish joins its parts in their order.
 #include <math.h>

@@ -473,9 +473,10 @@ GRETA_API int greta_cuda_paged_append(greta_stream_t stream, const greta_paged_c
                                       const void *q, uint32_t ld_q, const void *k, uint32_t ld_k, const void *v, uint32_t ld_v, uint32_t heads, void *q_out,
                                       int q_fmt, uint32_t ld_q_out);
 /* o = softmax(scale q k^T) v of every new row over the positions up to its own, with window > 0 over the last `window` of them.  q and o
- * [tokens][heads][dim], both of type q_fmt: GRETA_FMT_F32 (products and sums keep fp32 precision), or the cache's type (probabilities are
- * rounded to it, the rest is fp32).  heads: a multiple of kv_heads; scale: above 0, at most 2e38.  The new rows' keys and values are in the cache already (greta_cuda_paged_append).  What
- * lies behind a row's position, or in front of its window, does not reach it whatever it is.  Rows without keys are zeros.  o and q do not overlap.
+ * [tokens][heads][dim], both of type q_fmt: GRETA_FMT_F32 (products and sums keep fp32 precision; over fp16 caches weights
+ * below 2^-18 of a row's largest are off by up to 2^-40 of it), or the cache's type (probabilities are rounded to it, the rest is fp32).  heads: a multiple of kv_heads; scale: above 0, at most 2e38.  The new rows' keys and values are in the cache already (greta_cuda_paged_append).  What
+ * lies behind a row's position, or in front of its window, does not reach it whatever it is.  Rows without keys are zeros.  o and q do not
+ * overlap (columns of one buffer do not).
  * workspace: greta_cuda_paged_attn_workspace_bytes(dim) bytes, 16-byte aligned, its first 64 KB zero before the first call; one serves every
  * shape, one call at a time.  Waits in the kernels are bounded; one that gave up shows in greta_cuda_gemm_segments_status, and the workspace is cleared again before the
  * next call.
