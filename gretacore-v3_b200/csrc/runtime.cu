@@ -228,6 +228,8 @@ int greta_cuda_memcpy_2d_d2h_sync(void *dst, size_t dst_pitch, const void *src, 
 }
 int greta_cuda_memcpy_h2d_sync(void *dst, const void *src, size_t bytes) {
   GRETA_CUDA_TRY(cudaMemcpy(dst, src, bytes, cudaMemcpyHostToDevice));
+  // From pageable memory it returns when the last piece is staged; the streams made here do not wait for the one that still carries it.
+  GRETA_CUDA_TRY(cudaStreamSynchronize(cudaStreamLegacy));
   return GRETA_OK;
 }
 int greta_cuda_memcpy_d2h_sync(void *dst, const void *src, size_t bytes) {
