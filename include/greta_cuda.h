@@ -86,7 +86,7 @@ GRETA_API int greta_cuda_memcpy_2d_d2d(void *dst, size_t dst_pitch, const void *
                                        greta_stream_t stream);
 /* height rows of width bytes from a pitched device array to a pitched host array; blocks. */
 GRETA_API int greta_cuda_memcpy_2d_d2h_sync(void *dst, size_t dst_pitch, const void *src, size_t src_pitch, size_t width, size_t height);
-/* Both block: what is called behind them, on any stream, sees the bytes. */
+/* Blocks: what is called behind it, on any stream, sees the bytes. */
 GRETA_API int greta_cuda_memcpy_h2d_sync(void *dst, const void *src, size_t bytes);
 /* Bytes of the current device's memory that are free, and all of it. */
 GRETA_API int greta_cuda_mem_info(size_t *free_bytes, size_t *total_bytes);
